@@ -29,7 +29,7 @@
 extern "C" {
 #endif
 
-#define RECAP_B200_ABI_VERSION 8
+#define RECAP_B200_ABI_VERSION 9
 
 #define RECAP_OK 0
 #define RECAP_ERR_SHAPE 1
@@ -44,6 +44,17 @@ extern "C" {
 #define RECAP_STATUS_TIMEOUT_SOFTMAX 103
 #define RECAP_STATUS_TIMEOUT_PRODUCER 104
 #define RECAP_STATUS_TIMEOUT_SELFTEST 106 /* recap_wait_selftest only */
+
+/* element types and norms of recap_rotate_qk and recap_norm_rows */
+#define RECAP_TYPE_BF16 0
+#define RECAP_TYPE_F16 1
+#define RECAP_TYPE_F32 2
+#define RECAP_NORM_NONE 0
+#define RECAP_NORM_RMS 1
+#define RECAP_NORM_LAYER 2
+#define RECAP_NORM_RMS_ACROSS 3 /* recap_rotate_qk only: over all heads of a token */
+#define RECAP_MAX_AXES 4
+#define RECAP_MAX_PAIRS 128
 
 int recap_abi_version(void);
 
@@ -321,6 +332,77 @@ int recap_push_heads(const void* src, int tokens, int heads, int D, int rank, in
  * are multiples of 8 elements.  No counterpart in the reference. */
 int recap_scatter_rows(const void* src, int banks, int S, int D, void* const* out_ranks, int n_ranks,
                        int tokens_per_rank, int64_t out_bank_stride, int64_t out_row_stride, void* stream);
+
+/* Rotary positions of several axes (host struct, copied by the call).  Pair p in [0, pairs)
+ * turns by (position[axis[p]] * turns[p] + phase[p]) / 2^64 of a full turn, in wrapping 64-bit
+ * arithmetic.  halves 0: pair p is values 2p and 2p + 1; 1: values p and pairs + p (pairs a
+ * multiple of 4).  Values past 2 * pairs are not turned.  With a grid (video_tokens =
+ * product of grid[0 .. axes), > 0) token n has the grid coordinates of n - video_offset, the last
+ * axis fastest, and tokens outside it are not turned; with video_tokens 0 the positions come with the
+ * call. */
+typedef struct recap_rotary {
+  int32_t axes, pairs, halves, reserved;
+  int32_t grid[RECAP_MAX_AXES];
+  int64_t video_offset, video_tokens;
+  uint64_t turns[RECAP_MAX_PAIRS];
+  uint64_t phase[RECAP_MAX_PAIRS];
+  uint8_t axis[RECAP_MAX_PAIRS];
+} recap_rotary;
+
+/* Operands of recap_rotate_qk (host struct).  q and k [batch, heads, S, D] with D contiguous and
+ * element strides (b, h, s) in strides[0 .. 2] and [3 .. 5]; q_out and k_out likewise with strides
+ * [6 .. 8] and [9 .. 11]; k and k_out NULL with k_heads 0.  An output may be its input; otherwise
+ * it must not overlap either input.  Every base is 16-byte aligned, every stride a multiple of 16
+ * bytes, D a multiple of 8 up to 256.  out_type is in_type or bf16.
+ *   positions       int32 or int64 (position_bits 32 or 64) [batch, S, axes] with element strides
+ *                   position_strides (b, s, axis), or NULL with position_bits 0 (grid, or no turn)
+ *   first_token     the place in the grid's sequence of token 0 of this call
+ *   *_weight, *_bias  [D] of weight_type (RMS_ACROSS: weight [heads, D], at most 256 lanes of rows,
+ *                   that is heads <= 256, 128, 64 for D <= 64, 128, 256); NULL: none.  bias: layer norm only */
+typedef struct recap_rotate_qk_args {
+  const void *q, *k;
+  void *q_out, *k_out;
+  int64_t strides[12];
+  const void* positions;
+  int64_t position_strides[3];
+  int64_t first_token;
+  const void *q_weight, *q_bias, *k_weight, *k_bias;
+  int32_t batch, q_heads, k_heads, S, D, in_type, out_type, norm, weight_type, position_bits;
+  float q_eps, k_eps;
+} recap_rotate_qk_args;
+
+/* Query/key norm and rotary positions in one pass (the step between a video transformer's
+ * projections and Operator.attend, done in the reference by the model processors, e.g.
+ * recap/models/hunyuan.py): norm over each head (or all heads of a token), then the turn of
+ * `rotary` (NULL: none), in fp32, rounded once.  Empty calls (batch or S 0) launch nothing. */
+int recap_rotate_qk(const recap_rotate_qk_args* args, const recap_rotary* rotary, void* stream);
+
+/* Operands of recap_norm_rows (host struct).  x [batch, S, C] of x_type; branch (nullable) and h of
+ * h_type, which is x_type or, for fp32 x, bf16 or fp16; x_out of x_type.  C contiguous, a multiple of 8
+ * up to 16384; element strides (b, s): strides[0 .. 1] x, [2 .. 3] branch, [4 .. 5] x_out, [6 .. 7] h,
+ * multiples of 16 bytes, bases 16-byte aligned.  An output may be its input of the same type; otherwise
+ * it must not overlap an input.
+ *   scale, shift, gate  of mod_type (nullable each) with element strides (b, s) in mod_strides
+ *                       [0 .. 1], [2 .. 3], [4 .. 5]; 0 where one vector serves every sample or token
+ *   weight, bias, branch_weight, branch_bias  [C] (nullable each) of weight_type, branch_weight_type
+ *   norm, branch_norm   RECAP_NORM_NONE, _RMS or _LAYER */
+typedef struct recap_norm_rows_args {
+  const void *x, *branch;
+  void *x_out, *h;
+  int64_t strides[8];
+  const void *scale, *shift, *gate;
+  int64_t mod_strides[6];
+  const void *weight, *bias, *branch_weight, *branch_bias;
+  int32_t batch, S, C, x_type, h_type, norm, branch_norm, weight_type, branch_weight_type, mod_type;
+  float eps, branch_eps;
+} recap_norm_rows_args;
+
+/* The norm before a transformer block and, with a branch, the gate and residual sum after one:
+ *   x_out = x + gate (branch_norm(branch) branch_weight + branch_bias)       (branch given)
+ *   h = (norm(x or x_out) weight + bias) (1 + scale) + shift                 (norm given)
+ * in fp32, each output rounded once (h from the unrounded x_out).  The reference leaves these to the
+ * model's own blocks.  Empty calls (batch or S 0) launch nothing. */
+int recap_norm_rows(const recap_norm_rows_args* args, void* stream);
 
 #ifdef __cplusplus
 }

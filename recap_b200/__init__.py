@@ -7,6 +7,7 @@ ABI of ``include/recap_b200.h`` (``librecap_b200.so``).  Build the library with
 ``python -m recap_b200.build``.
 """
 
+from .block import AxialRotary, Norm, gated_residual, modulated_norm, rotate_qk
 from .config import OperatorConfig, keep_blocks
 from .host_banks import HostBankOperator
 from .operator import EXACT, REFRESH, SPARSE, DetailBank, Operator
@@ -16,13 +17,18 @@ __all__ = [
     "EXACT",
     "REFRESH",
     "SPARSE",
+    "AxialRotary",
     "DetailBank",
     "HostBankOperator",
     "Layout",
+    "Norm",
     "Operator",
     "OperatorConfig",
     "SparseAttention",
     "SparseGeometry",
+    "gated_residual",
     "hilbert_permutation",
     "keep_blocks",
+    "modulated_norm",
+    "rotate_qk",
 ]

@@ -1,0 +1,526 @@
+"""What stands around the attention call in a video transformer block.
+
+Between the projections and ``Operator.attend`` the models normalise queries and keys and
+turn them by rotary positions over (time, height, width); before and after the block stand
+a norm with scale and shift, a gate and a residual sum.  The reference leaves these steps to
+the model processors (recap/models/{cogvideox,wan,hunyuan}.py) and the models' own blocks;
+here each is one pass over its rows, in the kernels of ``librecap_b200.so``:
+
+``rotate_qk``       query/key norm and rotary positions (``AxialRotary``);
+``modulated_norm``  the norm before a block: ``norm(x) (1 + scale) + shift``;
+``gated_residual``  after a block: ``residual + gate * branch``, with the next block's
+                    modulated norm of the sum on the way.
+
+They compute in fp32 and round each output once.  Tensors are bf16, fp16 or fp32 on one
+CUDA device, rows contiguous in their last dim, bases and strides multiples of 16 bytes
+(``ValueError`` otherwise); the kernels run on the current stream of that device.  There is
+no backward pass, as there is none of ``Operator.attend``: inputs that require a gradient
+while gradients are being recorded raise ``RuntimeError``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+from dataclasses import dataclass
+from typing import Sequence
+
+import torch
+
+from . import _lib
+
+MAX_AXES = 4
+MAX_PAIRS = 128
+
+# The host structs of include/recap_b200.h as packed bytes: filling one and passing it by address
+# costs a fraction of converting thirty ctypes arguments, which a call on few tokens feels.
+_ROTATE_ARGS = struct.Struct("<4Q12qQ3qq4Q10i2f")
+_NORM_ARGS = struct.Struct("<4Q8q3Q6q4Q10i2f")
+
+_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_KINDS = {"rms": 1, "layer": 2}
+_RMS_ACROSS = 3
+
+
+class _RotaryStruct(ctypes.Structure):
+    _fields_ = [("axes", ctypes.c_int32), ("pairs", ctypes.c_int32), ("halves", ctypes.c_int32),
+                ("reserved", ctypes.c_int32), ("grid", ctypes.c_int32 * MAX_AXES), ("video_offset", ctypes.c_int64),
+                ("video_tokens", ctypes.c_int64), ("turns", ctypes.c_uint64 * MAX_PAIRS),
+                ("phase", ctypes.c_uint64 * MAX_PAIRS), ("axis", ctypes.c_uint8 * MAX_PAIRS)]
+
+
+def _per_axis(value, n: int, what: str) -> tuple[float, ...]:
+    values = tuple(float(v) for v in value) if isinstance(value, (tuple, list)) else (float(value),) * n
+    if len(values) != n:
+        raise ValueError(f"{what} needs one value, or one for each of the {n} axes")
+    if not all(math.isfinite(v) for v in values):
+        raise ValueError(f"{what} must be finite")
+    return values
+
+
+class AxialRotary:
+    """Rotary positions of one to four axes.
+
+    ``axis_dims``: how many of the ``head_dim`` values each axis turns (even numbers, in the
+    order of the axes); values past their sum are not turned.  Pair ``i`` of axis ``a`` turns
+    by ``(position[a] * scale[a] + start[a]) * theta[a] ** (-2 i / axis_dims[a])``; with
+    ``ladder="shared"`` the exponent runs over all axes together, ``-2 p / sum(axis_dims)``
+    for the p-th pair of the head.  ``pairs``: ``"interleaved"`` pairs values 2p and 2p + 1,
+    ``"halves"`` values p and p + sum(axis_dims) / 2.
+
+    With ``grid`` (for video (frames, height, width), the last axis fastest) the positions are
+    the grid coordinates of the token index, and the ``text_tokens`` before (``text_first``)
+    or after the grid are not turned: the native token order of ``Layout``.  Without it the
+    positions come with each call as an integer tensor, of any size: angles are kept as
+    64-bit fractions of a turn, so a far position turns as exactly as a near one.
+
+    The object holds numbers on the host only: it serves every device, stream and graph.
+    """
+
+    def __init__(self, head_dim: int, axis_dims: Sequence[int], *, theta=10000.0, grid: Sequence[int] | None = None,
+                 text_tokens: int = 0, text_first: bool = False, pairs: str = "interleaved", ladder: str = "axis",
+                 scale=1.0, start=0.0):
+        dims = tuple(int(d) for d in axis_dims)
+        n = len(dims)
+        if not 1 <= n <= MAX_AXES:
+            raise ValueError(f"rotary positions have 1 to {MAX_AXES} axes")
+        if any(d < 2 or d % 2 for d in dims) or sum(dims) > int(head_dim):
+            raise ValueError("axis_dims must be even, positive and sum to at most head_dim")
+        if head_dim % 8 or not 8 <= head_dim <= 2 * MAX_PAIRS:
+            raise ValueError(f"head_dim must be a multiple of 8 up to {2 * MAX_PAIRS}")
+        if pairs not in ("interleaved", "halves"):
+            raise ValueError(f"unknown pairs {pairs!r}")
+        if ladder not in ("axis", "shared"):
+            raise ValueError(f"unknown ladder {ladder!r}")
+        if pairs == "halves" and sum(dims) % 8:
+            raise ValueError("halves need a multiple of 8 turned values")
+        thetas = _per_axis(theta, n, "theta")
+        if min(thetas) <= 0:
+            raise ValueError("theta must be positive")
+        if ladder == "shared" and len(set(thetas)) > 1:
+            raise ValueError("a shared ladder has one theta")
+        scales, starts = _per_axis(scale, n, "scale"), _per_axis(start, n, "start")
+        if text_tokens < 0 or (grid is None and (text_tokens or text_first)):
+            raise ValueError("text_tokens belong to a grid and are not negative")
+        self.head_dim, self.axis_dims, self.pairs, self.ladder = int(head_dim), dims, pairs, ladder
+        self.text_tokens, self.text_first = int(text_tokens), bool(text_first)
+        self.grid = None
+        self.sequence_tokens = None
+        c = _RotaryStruct(axes=n, pairs=sum(dims) // 2, halves=pairs == "halves")
+        if grid is not None:
+            self.grid = tuple(int(g) for g in grid)
+            if len(self.grid) != n or min(self.grid) < 1 or math.prod(self.grid) >= 2**31:
+                raise ValueError("grid needs one positive size for each axis and under 2^31 tokens")
+            c.grid[:n] = self.grid
+            c.video_tokens = math.prod(self.grid)
+            c.video_offset = self.text_tokens if text_first else 0
+            self.sequence_tokens = c.video_tokens + self.text_tokens
+        p = 0
+        for axis, d in enumerate(dims):
+            for i in range(d // 2):
+                power = 2.0 * p / sum(dims) if ladder == "shared" else 2.0 * i / d
+                frequency = thetas[axis] ** -power / (2.0 * math.pi)  # turns for each unit of position
+                c.turns[p] = round(math.fmod(frequency * scales[axis], 1.0) * 2.0**64) % 2**64
+                c.phase[p] = round(math.fmod(frequency * starts[axis], 1.0) * 2.0**64) % 2**64
+                c.axis[p] = axis
+                p += 1
+        self._struct = c
+        self._address = ctypes.addressof(c)
+
+
+@dataclass
+class Norm:
+    """A norm over the last dim: ``"rms"`` (x / sqrt(mean x^2 + eps)) or ``"layer"`` (mean taken off
+    first, population variance), times ``weight``, plus ``bias`` (layer norms only).  With
+    ``across_heads`` (rms, ``rotate_qk`` only) the mean runs over all heads of a token and the
+    weight has a value for each head and dim."""
+
+    kind: str
+    weight: torch.Tensor | None = None
+    bias: torch.Tensor | None = None
+    eps: float = 1e-6
+    across_heads: bool = False
+
+    def __post_init__(self) -> None:
+        if self.kind not in _KINDS:
+            raise ValueError(f"unknown norm {self.kind!r}")
+        if self.bias is not None and self.kind != "layer":
+            raise ValueError("only a layer norm has a bias")
+        if self.across_heads and self.kind != "rms":
+            raise ValueError("across_heads is a root mean square norm")
+        if not self.eps >= 0.0 or math.isinf(self.eps):
+            raise ValueError("eps must be finite and not negative")
+
+    @property
+    def code(self) -> int:
+        return _RMS_ACROSS if self.across_heads else _KINDS[self.kind]
+
+
+def _refuse_gradients(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("this operator has no backward pass: call it under torch.no_grad()")
+
+
+def _type(dtype: torch.dtype, what: str) -> int:
+    code = _TYPES.get(dtype)
+    if code is None:
+        raise ValueError(f"{what} must be bfloat16, float16 or float32, not {dtype}")
+    return code
+
+
+def _param(t: torch.Tensor | None, n: int, device, what: str) -> int:
+    """Address of an optional parameter vector of ``n`` contiguous values."""
+    if t is None:
+        return 0
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what} must be {n} contiguous values")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the rows on {device}")
+    return t.data_ptr()
+
+
+def _norm_params(norm: Norm | None, n: int, device, what: str) -> tuple[int, int, int]:
+    """(weight address, bias address, their type) of an optional norm."""
+    if norm is None:
+        return 0, 0, 0
+    weight, bias = norm.weight, norm.bias
+    _refuse_gradients(weight, bias)
+    code = 0
+    if weight is not None:
+        code = _type(weight.dtype, what)
+        if bias is not None and bias.dtype != weight.dtype:
+            raise ValueError(f"{what} weight and bias differ in type")
+    elif bias is not None:
+        code = _type(bias.dtype, what)
+    return _param(weight, n, device, f"{what} weight"), _param(bias, n, device, f"{what} bias"), code
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """First byte and the byte past the last of what a tensor's elements span."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
+    """Whether two tensors share no element: their spans are apart, or they are the same rows
+    of one packed buffer at different places of each token (``[b, s, 3, h, d]`` projections)."""
+    if x.numel() == 0 or y.numel() == 0:
+        return True
+    (x0, x1), (y0, y1) = _extent(x), _extent(y)
+    if x1 <= y0 or y1 <= x0:
+        return True
+    if x.dim() != 4 or x.stride() != y.stride() or x.dtype != y.dtype:
+        return False
+    sb, sh, ss, _ = x.stride()
+    wide = (max(x.shape[1], y.shape[1]) - 1) * sh + x.shape[3]
+    if ss <= 0 or (x.shape[0] > 1 and sb % ss):
+        return False
+    return wide <= (y0 - x0) // x.element_size() % ss <= ss - wide
+
+
+def _same(x: torch.Tensor, y: torch.Tensor) -> bool:
+    return x.data_ptr() == y.data_ptr() and x.stride() == y.stride() and x.dtype == y.dtype
+
+
+def _check_outputs(outs: Sequence[torch.Tensor], inputs: Sequence[torch.Tensor]) -> None:
+    """Outputs hold each element once, may be the input of the same place in the list, and
+    otherwise overlap neither an input nor one another."""
+    for i, o in enumerate(outs):
+        if any(n > 1 and s == 0 for n, s in zip(o.shape, o.stride())):
+            raise ValueError("an output cannot be an expanded tensor")
+        for j, x in enumerate(inputs):
+            if not (i == j and _same(o, x)) and not _apart(o, x):
+                raise ValueError("an output overlaps an input (it may only be that input itself)")
+        for p in outs[i + 1:]:
+            if not _apart(o, p):
+                raise ValueError("the outputs overlap")
+
+
+def _run(name: str, device: torch.device, *args) -> None:
+    """Call an entry point with ``device`` current, on its current stream."""
+    if torch.cuda.current_device() == device.index:
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        return
+    with torch.cuda.device(device):
+        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+
+
+def rotate_qk(
+    query: torch.Tensor,
+    key: torch.Tensor | None,
+    rotary: AxialRotary | None = None,
+    *,
+    query_norm: Norm | None = None,
+    key_norm: Norm | None = None,
+    positions: torch.Tensor | None = None,
+    first_token: int = 0,
+    out_dtype: torch.dtype | None = None,
+    out: tuple[torch.Tensor, torch.Tensor | None] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Normalise queries and keys and turn them by rotary positions, in one pass.
+
+    ``query`` ``[batch, heads, sequence, dim]`` and ``key`` (the same with its own head count,
+    or None) in native token order, dim contiguous, a multiple of 8 up to 256, other strides free.
+    ``rotary`` None: norm only.  ``positions`` (a rotary without a grid): int32 or int64
+    ``[batch or 1, sequence, axes]`` or ``[sequence, axes]``.  ``first_token``: the place of token 0 in
+    the grid's sequence, for a shard or a chunk of it.  The norms are of one kind; a norm across heads
+    takes at most 256, 128 and 64 heads of up to 64, 128 and 256 dims.
+
+    Returns new tensors in the inputs' token order, of their dtype or of ``out_dtype`` bfloat16; ``out``
+    gives them instead: the inputs themselves (in place) or tensors that do not overlap them."""
+    if query.dim() != 4 or query.stride(3) != 1 and query.shape[3] > 1:
+        raise ValueError("query must be [batch, heads, sequence, dim] with dim contiguous")
+    b, hq, s, d = query.shape
+    hk = 0
+    if key is not None:
+        if key.dim() != 4 or key.stride(3) != 1 and key.shape[3] > 1:
+            raise ValueError("key must be [batch, heads, sequence, dim] with dim contiguous")
+        hk = key.shape[1]
+        if key.shape[0] != b or key.shape[2] != s or key.shape[3] != d:
+            raise ValueError("query and key differ in batch, sequence or dim")
+        if key.dtype != query.dtype or key.device != query.device:
+            raise ValueError("query and key differ in dtype or device")
+        if hk < 1:
+            raise ValueError("key has no heads")
+    if d % 8 or not 8 <= d <= 256 or hq < 1:
+        raise ValueError("dim must be a multiple of 8 up to 256, and heads positive")
+    device = query.device
+    in_type = _type(query.dtype, "query")
+    _refuse_gradients(query, key)
+    out_type = in_type
+    if out_dtype is not None and out_dtype != query.dtype:
+        if out_dtype != torch.bfloat16:
+            raise ValueError("out_dtype is the inputs' dtype or bfloat16")
+        out_type = 0
+
+    if query_norm is None and key_norm is None:
+        code = 0
+    else:
+        if query_norm is None or (key is not None and key_norm is None):
+            raise ValueError("query and key are both normalised or neither")
+        code = query_norm.code
+        if key is not None and key_norm.code != code:
+            raise ValueError("the query's and the key's norm differ in kind")
+        if code == _RMS_ACROSS and max(hq, hk) > (256 if d <= 64 else 128 if d <= 128 else 64):
+            raise ValueError(f"too many heads of {d} dims for a norm across heads")
+    across = code == _RMS_ACROSS
+    qw, qb, weight_type = _norm_params(query_norm, hq * d if across else d, device, "query norm")
+    kw, kb, k_type = _norm_params(key_norm if key is not None else None, hk * d if across else d, device, "key norm")
+    if (kw or kb) and (qw or qb) and k_type != weight_type:
+        raise ValueError("the norms' weights differ in type")
+    if kw or kb:
+        weight_type = k_type
+
+    address = bits = at = 0
+    pb = ps = pa = 0
+    if rotary is not None:
+        address = rotary._address
+        if rotary.head_dim != d:
+            raise ValueError(f"rotary positions of {rotary.head_dim} dims on heads of {d}")
+        if rotary.grid is not None:
+            if positions is not None:
+                raise ValueError("positions are given by the rotary's grid")
+            if first_token < 0 or first_token + s > rotary.sequence_tokens:
+                raise ValueError(f"tokens {first_token}..{first_token + s} outside the sequence of "
+                                 f"{rotary.sequence_tokens}")
+        else:
+            if first_token:
+                raise ValueError("first_token belongs to a grid")
+            if positions is None:
+                raise ValueError("a rotary without a grid needs positions")
+            if positions.dtype == torch.int64:
+                bits = 64
+            elif positions.dtype == torch.int32:
+                bits = 32
+            else:
+                raise ValueError("positions must be int32 or int64")
+            shape, strides = positions.shape, positions.stride()
+            if len(shape) == 2:
+                shape, strides = (1, *shape), (0, *strides)
+            if len(shape) != 3 or shape[0] not in (1, b) or shape[1] != s or shape[2] != len(rotary.axis_dims):
+                raise ValueError("positions must be [batch or 1, sequence, axes]")
+            if positions.device != device:
+                raise ValueError(f"positions are on {positions.device}, the rows on {device}")
+            pb, ps, pa = strides if shape[0] == b else (0, strides[1], strides[2])
+            at = positions.data_ptr()
+    elif positions is not None or first_token:
+        raise ValueError("positions and first_token need a rotary")
+
+    if out is None:
+        q_out = torch.empty_like(query, dtype=out_dtype)
+        k_out = None if key is None else torch.empty_like(key, dtype=out_dtype)
+    else:
+        q_out, k_out = out
+        pairs = [(q_out, query)] if key is None else [(q_out, query), (k_out, key)]
+        for o, x in pairs:
+            if o is None or o.shape != x.shape or o.device != device or o.stride(3) != 1 and d > 1:
+                raise ValueError("out must match query and key, dim contiguous")
+            if o.dtype != q_out.dtype or (out_dtype is not None and o.dtype != out_dtype):
+                raise ValueError("out differs in dtype")
+        if q_out.dtype != query.dtype and q_out.dtype != torch.bfloat16:
+            raise ValueError("out has the inputs' dtype or bfloat16")
+        out_type = _TYPES[q_out.dtype]
+        _check_outputs([o for o, _ in pairs], [x for _, x in pairs])
+    if not query.is_cuda:
+        raise ValueError("rotate_qk runs on CUDA tensors only")
+    if b == 0 or s == 0:
+        return q_out, k_out
+    qs, qos = query.stride(), q_out.stride()
+    if key is None:
+        k_ptr = ko_ptr = 0
+        ks = kos = (0, 0, 0)
+    else:
+        k_ptr, ko_ptr, ks, kos = key.data_ptr(), k_out.data_ptr(), key.stride(), k_out.stride()
+    args = _ROTATE_ARGS.pack(
+        query.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qos[0], qos[1],
+        qos[2], kos[0], kos[1], kos[2], at, pb, ps, pa, first_token, qw, qb, kw, kb, b, hq, hk, s, d, in_type, out_type,
+        code, weight_type, bits, query_norm.eps if query_norm is not None else 0.0,
+        key_norm.eps if key_norm is not None else 0.0)
+    _run("recap_rotate_qk", device, args, address)
+    return q_out, k_out
+
+
+def _rows(t: torch.Tensor, like: torch.Tensor, what: str) -> tuple[int, int]:
+    """Element strides (batch, token) of rows ``[batch, tokens, channels]`` or ``[tokens, channels]``."""
+    if t.shape != like.shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
+    if t.device != like.device:
+        raise ValueError(f"{what} is on {t.device}, the rows on {like.device}")
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
+        raise ValueError(f"{what} needs contiguous channels")
+    return (0, st[0]) if len(st) == 2 else (st[0], st[1])
+
+
+def _modulation(t: torch.Tensor | None, like: torch.Tensor, what: str) -> tuple[int, int, int]:
+    """Address and element strides (batch, token; 0 where shared) of a modulation: one vector
+    ``[channels]``, or the rows' dims with size 1 where it is shared."""
+    if t is None:
+        return 0, 0, 0
+    shape, st, rows = t.shape, t.stride(), like.shape
+    if t.device != like.device:
+        raise ValueError(f"{what} is on {t.device}, the rows on {like.device}")
+    if shape[-1:] != rows[-1:] or (st[-1] != 1 and shape[-1] > 1):
+        raise ValueError(f"{what} needs {rows[-1]} contiguous channels")
+    if len(shape) == 1:
+        return t.data_ptr(), 0, 0
+    if len(shape) != len(rows) or any(m != n and m != 1 for m, n in zip(shape, rows)):
+        raise ValueError(f"{what} has shape {tuple(shape)}, which does not spread over {tuple(rows)}")
+    steps = [0 if m == 1 else step for m, step in zip(shape, st)]
+    return t.data_ptr(), 0 if len(shape) == 2 else steps[0], steps[-2]
+
+
+def _norm_rows(what: str, x, branch, gate, branch_norm, norm, scale, shift, x_out, h, h_dtype):
+    if x.dim() not in (2, 3):
+        raise ValueError("rows are [batch, tokens, channels] or [tokens, channels]")
+    c = x.shape[-1]
+    if c % 8 or not 8 <= c <= 16384:
+        raise ValueError("channels must be a multiple of 8 up to 16384")
+    device = x.device
+    x_type, h_type = _type(x.dtype, "rows"), _type(h_dtype, "the norm's output")
+    if h_type != x_type and x_type != 2:
+        raise ValueError("only float32 rows have a norm or a branch of another type")
+    _refuse_gradients(x, branch, gate, scale, shift)
+    xs = _rows(x, x, "rows")
+    bs = (0, 0) if branch is None else _rows(branch, x, "branch")
+    mods = [t for t in (scale, shift, gate) if t is not None]
+    mod_type = _type(mods[0].dtype, "modulations") if mods else 0
+    if any(t.dtype != mods[0].dtype for t in mods):
+        raise ValueError("scale, shift and gate differ in type")
+    sc, sh, ga = (_modulation(t, x, n) for t, n in ((scale, "scale"), (shift, "shift"), (gate, "gate")))
+    for n in (norm, branch_norm):
+        if n is not None and n.across_heads:
+            raise ValueError("a norm across heads belongs to rotate_qk")
+    w, wb, w_type = _norm_params(norm, c, device, "norm")
+    bw, bb, b_type = _norm_params(branch_norm, c, device, "branch norm")
+    outs, ins = [], []
+    xos = hs = (0, 0)
+    if branch is not None:
+        if x_out is None:
+            x_out = torch.empty_like(x)
+        else:
+            outs.append(x_out)
+            ins.append(x)
+            if x_out.dtype != x.dtype:
+                raise ValueError("the sum has the residual's dtype")
+        xos = _rows(x_out, x, "out")
+    if norm is not None:
+        if h is None:
+            h = torch.empty_like(x if branch is None else branch, dtype=h_dtype)
+        else:
+            outs.append(h)
+            ins.append(x if branch is None else branch)
+            if h.dtype != h_dtype:
+                raise ValueError("the norm's out differs in dtype")
+        hs = _rows(h, x, "out")
+    if outs:
+        every = [t for t in (x, branch) if t is not None]
+        _check_outputs(outs, ins)
+        for o, mine in zip(outs, ins):
+            for t in every + [t for t in (scale, shift, gate) if t is not None]:
+                if t is not mine and not _apart(o, t):
+                    raise ValueError("an output overlaps an input (it may only be that input itself)")
+    if not x.is_cuda:
+        raise ValueError(f"{what} runs on CUDA tensors only")
+    b, s = (1, x.shape[0]) if x.dim() == 2 else (x.shape[0], x.shape[1])
+    if b == 0 or s == 0:
+        return x_out, h
+    args = _NORM_ARGS.pack(
+        x.data_ptr(), 0 if branch is None else branch.data_ptr(), 0 if branch is None else x_out.data_ptr(),
+        0 if norm is None else h.data_ptr(), *xs, *bs, *xos, *hs, sc[0], sh[0], ga[0], *sc[1:], *sh[1:], *ga[1:], w, wb,
+        bw, bb, b, s, c, x_type, h_type, 0 if norm is None else norm.code,
+        0 if branch_norm is None else branch_norm.code, w_type, b_type, mod_type, 0.0 if norm is None else norm.eps,
+        0.0 if branch_norm is None else branch_norm.eps)
+    _run("recap_norm_rows", device, args)
+    return x_out, h
+
+
+def modulated_norm(
+    x: torch.Tensor,
+    norm: Norm,
+    *,
+    scale: torch.Tensor | None = None,
+    shift: torch.Tensor | None = None,
+    out_dtype: torch.dtype | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """The norm before a block: ``norm(x) (1 + scale) + shift``.
+
+    ``x`` ``[batch, tokens, channels]`` or ``[tokens, channels]``, channels contiguous, a multiple of 8 up
+    to 16384.  ``scale`` and ``shift``, of one dtype: ``[channels]``, or the dims of ``x`` with size 1
+    where they are shared (``[batch, 1, channels]`` of a sample, ``[batch, tokens, channels]`` of every
+    token).  The result has the dtype of ``x``, or for float32 rows ``out_dtype``; ``out`` may be ``x``
+    itself or a tensor that does not overlap the inputs."""
+    if out is not None and out_dtype is None:
+        out_dtype = out.dtype
+    return _norm_rows("modulated_norm", x, None, None, None, norm, scale, shift, None, out,
+                      x.dtype if out_dtype is None else out_dtype)[1]
+
+
+def gated_residual(
+    residual: torch.Tensor,
+    branch: torch.Tensor,
+    gate: torch.Tensor | None = None,
+    *,
+    branch_norm: Norm | None = None,
+    norm: Norm | None = None,
+    scale: torch.Tensor | None = None,
+    shift: torch.Tensor | None = None,
+    out: tuple[torch.Tensor | None, torch.Tensor | None] | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """After a block: the sum ``x = residual + gate * branch_norm(branch)`` and, with ``norm``, the
+    next block's input ``norm(x) (1 + scale) + shift`` (of the sum before it is rounded).
+
+    ``residual`` and ``branch`` are rows as in ``modulated_norm``; the branch has the residual's dtype, or
+    is bf16 or fp16 beside a float32 residual.  ``gate``, ``scale`` and ``shift``, of one dtype, spread
+    over the rows as there.  Returns (sum of the residual's dtype, norm of the branch's dtype or None);
+    ``out`` gives either or both: the sum may be the residual itself, the norm the branch itself."""
+    if norm is None and (scale is not None or shift is not None):
+        raise ValueError("scale and shift belong to a norm")
+    x_out, h = out if out is not None else (None, None)
+    if norm is None and h is not None:
+        raise ValueError("out of a norm that is not asked for")
+    return _norm_rows("gated_residual", residual, branch, gate, branch_norm, norm, scale, shift, x_out, h, branch.dtype)

@@ -681,3 +681,159 @@ int recap_scatter_rows(const void* src, int banks, int S, int D, void* const* ou
 }
 
 }  // extern "C"
+
+static_assert(sizeof(recap_rotary) == 2224 && sizeof(recap_rotate_qk_args) == 248 &&
+                  sizeof(recap_norm_rows_args) == 248,
+              "the bindings fill these structs by their layout");
+
+// Whether rows at `p` may be read or written 16 bytes at a time: base and element strides of
+// every dim of more than one element.
+static bool wide_ok(const void* p, const int64_t* strides, const int (&sizes)[3], int type) {
+  if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15)) return false;
+  for (int i = 0, j = 0; i < 3; ++i) {
+    if (sizes[i] == 0) continue;  // a dim these rows do not have
+    if (sizes[i] > 1 && strides[j] % (type == kTypeF32 ? 4 : 8)) return false;
+    ++j;
+  }
+  return true;
+}
+static bool param_ok(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+static bool type_ok(int t) { return t == kTypeBf16 || t == kTypeF16 || t == kTypeF32; }
+
+extern "C" {
+
+int recap_rotate_qk(const recap_rotate_qk_args* p, const recap_rotary* rotary, void* stream) {
+  if (p == nullptr || p->batch < 0 || p->S < 0 || p->q_heads <= 0 || p->k_heads < 0 || p->D <= 0 || p->D > 256 ||
+      p->D % 8 || p->norm < kNormNone || p->norm > kNormRmsAcross || !type_ok(p->in_type) || !type_ok(p->weight_type))
+    return kErrShape;
+  if (p->out_type != p->in_type && p->out_type != kTypeBf16) return kErrUnsupported;
+  if (p->norm == kNormRmsAcross &&
+      (p->q_heads > rotate_max_heads_across(p->D) || p->k_heads > rotate_max_heads_across(p->D)))
+    return kErrUnsupported;
+  RotateArgs a{};
+  if (rotary != nullptr) {
+    if (rotary->axes < 1 || rotary->axes > kMaxAxes || rotary->pairs < 0 || 2 * rotary->pairs > p->D ||
+        (rotary->halves && rotary->pairs % 4) || rotary->video_tokens < 0 || rotary->video_tokens > 2147483647)
+      return kErrShape;
+    const bool given = p->position_bits != 0;
+    if (given ? (p->position_bits != 32 && p->position_bits != 64) || p->positions == nullptr ||
+                    (reinterpret_cast<uintptr_t>(p->positions) % (p->position_bits / 8))
+              : rotary->video_tokens == 0)
+      return kErrShape;
+    a.axes = rotary->axes;
+    a.pairs = rotary->pairs;
+    a.halves = rotary->halves != 0;
+    a.video_offset = rotary->video_offset;
+    a.video_tokens = rotary->video_tokens;
+    int64_t n = 1;
+    for (int i = 0; i < a.axes; ++i) {
+      a.grid[i] = rotary->grid[i];
+      if (!given && a.grid[i] <= 0) return kErrShape;
+      n *= given ? 1 : a.grid[i];
+      if (n > 2147483647) return kErrShape;
+    }
+    if (!given && n != a.video_tokens) return kErrShape;
+    for (int i = 0; i < a.pairs; ++i) {
+      if (rotary->axis[i] >= a.axes) return kErrShape;
+      a.turns[i] = rotary->turns[i];
+      a.phase[i] = rotary->phase[i];
+      a.axis[i] = rotary->axis[i];
+    }
+    a.position_bits = p->position_bits;
+    a.positions = p->positions;
+    for (int i = 0; i < 3; ++i) a.position_stride[i] = p->position_strides[i];
+    a.first_token = p->first_token;
+  }
+  if (p->batch == 0 || p->S == 0) return kOk;
+  const void* x[2] = {p->q, p->k};
+  void* out[2] = {p->q_out, p->k_out};
+  const void* w[2] = {p->q_weight, p->k_weight};
+  const void* b[2] = {p->q_bias, p->k_bias};
+  a.heads[0] = p->q_heads;
+  a.heads[1] = p->k_heads;
+  a.eps[0] = p->q_eps;
+  a.eps[1] = p->k_eps;
+  for (int t = 0; t < 2; ++t) {
+    if (a.heads[t] == 0) continue;
+    const int sizes[3] = {p->batch, a.heads[t], p->S};
+    if (!wide_ok(x[t], p->strides + 3 * t, sizes, p->in_type) ||
+        !wide_ok(out[t], p->strides + 6 + 3 * t, sizes, p->out_type) ||
+        !param_ok(w[t]) || !param_ok(b[t]))
+      return kErrShape;
+    a.x[t] = x[t];
+    a.out[t] = out[t];
+    a.weight[t] = w[t];
+    a.bias[t] = b[t];
+    for (int i = 0; i < 3; ++i) {
+      a.x_stride[t][i] = p->strides[3 * t + i];
+      a.out_stride[t][i] = p->strides[6 + 3 * t + i];
+    }
+  }
+  a.batch = p->batch;
+  a.S = p->S;
+  a.D = p->D;
+  a.in_type = p->in_type;
+  a.out_type = p->out_type;
+  a.norm = p->norm;
+  a.weight_type = p->weight_type;
+  return launch_rotate(a, static_cast<cudaStream_t>(stream));
+}
+
+int recap_norm_rows(const recap_norm_rows_args* p, void* stream) {
+  if (p == nullptr || p->batch < 0 || p->S < 0 || p->C <= 0 || p->C % 8 || !type_ok(p->x_type) || !type_ok(p->h_type) ||
+      !type_ok(p->weight_type) || !type_ok(p->branch_weight_type) || !type_ok(p->mod_type) || p->norm < kNormNone ||
+      p->norm > kNormLayer || p->branch_norm < kNormNone || p->branch_norm > kNormLayer ||
+      static_cast<int64_t>(p->batch) * p->S > 2147483647)
+    return kErrShape;
+  if (p->C > norm_max_channels()) return kErrUnsupported;
+  if (p->h_type != p->x_type && p->x_type != kTypeF32) return kErrUnsupported;
+  const bool gate = p->branch != nullptr;
+  const bool norm = p->norm != kNormNone;
+  if (!gate && !norm) return kErrShape;
+  if (p->batch == 0 || p->S == 0) return kOk;
+  const int sizes[3] = {p->batch, p->S, 0};
+  if (!wide_ok(p->x, p->strides, sizes, p->x_type) ||
+      (gate && !wide_ok(p->branch, p->strides + 2, sizes, p->h_type)) ||
+      (gate && !wide_ok(p->x_out, p->strides + 4, sizes, p->x_type)) ||
+      (norm && !wide_ok(p->h, p->strides + 6, sizes, p->h_type)))
+    return kErrShape;
+  NormArgs a{};
+  const void* mod[3] = {p->scale, p->shift, p->gate};
+  for (int m = 0; m < 3; ++m) {
+    if (mod[m] != nullptr && !wide_ok(mod[m], p->mod_strides + 2 * m, sizes, p->mod_type)) return kErrShape;
+    a.mod[m] = mod[m];
+    a.mod_stride[m][0] = p->mod_strides[2 * m];
+    a.mod_stride[m][1] = p->mod_strides[2 * m + 1];
+  }
+  if (!param_ok(p->weight) || !param_ok(p->bias) || !param_ok(p->branch_weight) || !param_ok(p->branch_bias))
+    return kErrShape;
+  a.x = p->x;
+  a.branch = p->branch;
+  a.x_out = p->x_out;
+  a.h = p->h;
+  for (int i = 0; i < 2; ++i) {
+    a.x_stride[i] = p->strides[i];
+    a.branch_stride[i] = p->strides[2 + i];
+    a.x_out_stride[i] = p->strides[4 + i];
+    a.h_stride[i] = p->strides[6 + i];
+  }
+  a.weight = p->weight;
+  a.bias = p->bias;
+  a.branch_weight = p->branch_weight;
+  a.branch_bias = p->branch_bias;
+  a.eps = p->eps;
+  a.branch_eps = p->branch_eps;
+  a.batch = p->batch;
+  a.S = p->S;
+  a.C = p->C;
+  a.x_type = p->x_type;
+  a.h_type = p->h_type;
+  a.norm = p->norm;
+  a.branch_norm = p->branch_norm;
+  a.weight_type = p->weight_type;
+  a.branch_weight_type = p->branch_weight_type;
+  a.mod_type = p->mod_type;
+  return launch_norm_rows(a, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

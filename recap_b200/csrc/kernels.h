@@ -236,4 +236,51 @@ int launch_refresh_noalloc(RefreshArgs a, cudaStream_t s);
 int make_tmap_bf16(CUtensorMap* map, const void* base, uint64_t rows, uint64_t cols,
                    uint32_t box_rows);
 
+// ------------------------------------------------------------------ rows around the attention
+// Element types and norms of the row kernels (the values of the C ABI's RECAP_TYPE_* and
+// RECAP_NORM_*).
+enum : int { kTypeBf16 = 0, kTypeF16 = 1, kTypeF32 = 2 };
+enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2, kNormRmsAcross = 3 };
+constexpr int kMaxAxes = 4;
+constexpr int kMaxPairs = 128;
+
+struct RotateArgs {
+  const void* x[2];                     // q, k [batch, heads, S, D], D contiguous
+  void* out[2];
+  int64_t x_stride[2][3];               // elements (b, h, s)
+  int64_t out_stride[2][3];
+  int heads[2];                         // heads[1] 0: no k
+  const void* weight[2];                // norm weight [D], or [heads, D] across heads (nullable)
+  const void* bias[2];                  // layer norm bias [D] (nullable)
+  float eps[2];
+  int batch, S, D, in_type, out_type, norm, weight_type;
+  int position_bits;                    // 0: from the grid; 32, 64: integers at `positions`
+  const void* positions;
+  int64_t position_stride[3];           // elements (b, s, axis)
+  int64_t first_token, video_offset, video_tokens;  // the grid starts at token video_offset
+  int axes, pairs, halves;
+  int grid[kMaxAxes];
+  int split_log2[2], token_fast[2];     // set by launch_rotate
+  uint64_t turns[kMaxPairs];            // turns of the pair per position, times 2^64
+  uint64_t phase[kMaxPairs];
+  uint8_t axis[kMaxPairs];
+};
+int rotate_max_heads_across(int D);
+int launch_rotate(RotateArgs& a, cudaStream_t s);
+
+struct NormArgs {
+  const void* x;                        // [batch, S, C] input, or the residual
+  const void* branch;                   // [batch, S, C] block output (null: norm only)
+  void* x_out;                          // residual + gate * branch (with branch)
+  void* h;                              // modulated norm (null with norm none)
+  int64_t x_stride[2], branch_stride[2], x_out_stride[2], h_stride[2];  // elements (b, s)
+  const void* mod[3];                   // scale, shift, gate (nullable each)
+  int64_t mod_stride[3][2];             // elements (b, s), 0 where shared
+  const void *weight, *bias, *branch_weight, *branch_bias;  // [C] (nullable each)
+  float eps, branch_eps;
+  int batch, S, C, x_type, h_type, norm, branch_norm, weight_type, branch_weight_type, mod_type;
+};
+int norm_max_channels();
+int launch_norm_rows(const NormArgs& a, cudaStream_t s);
+
 }  // namespace recap

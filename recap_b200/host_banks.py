@@ -240,12 +240,12 @@ class HostBankOperator(Operator):
     # -- dispatch -------------------------------------------------------------------------
 
     @torch.no_grad()
-    def attend(self, layer_index: int, query, key, value):
+    def attend(self, layer_index: int, query, key, value, **turn):
         if self.kind not in (REFRESH, SPARSE):
-            return super().attend(layer_index, query, key, value)
+            return super().attend(layer_index, query, key, value, **turn)
         b, h, _, dim = query.shape
         if self._choose_residency(b * h, dim, query.device):
-            return super().attend(layer_index, query, key, value)
+            return super().attend(layer_index, query, key, value, **turn)
 
         ident = (self.stream, layer_index)
         bank = self.banks[self.stream][layer_index]
@@ -263,7 +263,7 @@ class HostBankOperator(Operator):
         self._prefetch_next(ident, slot)
         bank.value, bank.log_mass = slot.value, slot.log_mass
         try:
-            out = super().attend(layer_index, query, key, value)
+            out = super().attend(layer_index, query, key, value, **turn)
         finally:
             if self.kind == REFRESH:
                 self._write_back(slot, ident)

@@ -32,6 +32,7 @@ from dataclasses import dataclass, field, fields
 import torch
 
 from . import _lib
+from .block import AxialRotary, Norm, rotate_qk
 from .config import OperatorConfig
 from .sparse.attention import Launches, LayerInputs, SparseAttention, SparseGeometry
 from .sparse.layout import Layout, gather_rows, video_offset, video_permutation_i32
@@ -244,13 +245,25 @@ class Operator:
         query: torch.Tensor,
         key: torch.Tensor,
         value: torch.Tensor,
+        *,
+        rotary: AxialRotary | None = None,
+        query_norm: Norm | None = None,
+        key_norm: Norm | None = None,
+        positions: torch.Tensor | None = None,
     ) -> torch.Tensor:
-        """One attention call: ``[b, h, S, d]`` native order in, same shape/dtype out."""
+        """One attention call: ``[b, h, S, d]`` native order in, same shape/dtype out.
+
+        With ``rotary`` or the norms, ``query`` and ``key`` are the projections as they come:
+        they are normalised and turned first (``rotate_qk``), in new tensors."""
         if not (query.is_cuda and key.is_cuda and value.is_cuda):
             raise ValueError("recap_b200.Operator runs on CUDA tensors only")
         if query.shape != key.shape or key.shape != value.shape:
             raise ValueError("Q/K/V shapes differ")
         in_dtype = query.dtype
+        if rotary is not None or query_norm is not None or key_norm is not None or positions is not None:
+            query, key = rotate_qk(query, key, rotary, query_norm=query_norm, key_norm=key_norm, positions=positions,
+                                   out_dtype=torch.bfloat16)
+            self.launches.count += 1
         if in_dtype != torch.bfloat16:
             query, key, value = (t.to(torch.bfloat16) for t in (query, key, value))
         layer = self.layers[self.stream][layer_index]
