@@ -335,7 +335,7 @@ int recap_scatter_rows(const void* src, int banks, int S, int D, void* const* ou
 
 /* Rotary positions of several axes (host struct, copied by the call).  Pair p in [0, pairs)
  * turns by (position[axis[p]] * turns[p] + phase[p]) / 2^64 of a full turn, in wrapping 64-bit
- * arithmetic.  halves 0: pair p is values 2p and 2p + 1; 1: values p and pairs + p (pairs a
+ * arithmetic, of which the angle takes the top 32 bits (as does the phase).  halves 0: pair p is values 2p and 2p + 1; 1: values p and pairs + p (pairs a
  * multiple of 4).  Values past 2 * pairs are not turned.  With a grid (video_tokens =
  * product of grid[0 .. axes), > 0) token n has the grid coordinates of n - video_offset, the last
  * axis fastest, and tokens outside it are not turned; with video_tokens 0 the positions come with the

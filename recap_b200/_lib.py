@@ -116,6 +116,12 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(index: int) -> int:
+    """The cudaStream_t of a device's current stream, without a torch Stream object around it (what
+    the launch of a kernel of a few microseconds waits for)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def check(rc: int, what: str) -> None:
     if rc == RECAP_OK:
         return

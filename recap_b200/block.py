@@ -122,7 +122,8 @@ class AxialRotary:
                 power = 2.0 * p / sum(dims) if ladder == "shared" else 2.0 * i / d
                 frequency = thetas[axis] ** -power / (2.0 * math.pi)  # turns for each unit of position
                 c.turns[p] = round(math.fmod(frequency * scales[axis], 1.0) * 2.0**64) % 2**64
-                c.phase[p] = round(math.fmod(frequency * starts[axis], 1.0) * 2.0**64) % 2**64
+                # added to the top 32 bits of the product, which are cut: up makes up for down
+                c.phase[p] = (math.ceil(math.fmod(frequency * starts[axis], 1.0) * 2.0**32) % 2**32) << 32
                 c.axis[p] = axis
                 p += 1
         self._struct = c
@@ -154,6 +155,7 @@ class Norm:
 
     @property
     def code(self) -> int:
+        """The norm's RECAP_NORM_* value."""
         return _RMS_ACROSS if self.across_heads else _KINDS[self.kind]
 
 
@@ -171,31 +173,31 @@ def _type(dtype: torch.dtype, what: str) -> int:
     return code
 
 
-def _param(t: torch.Tensor | None, n: int, device, what: str) -> int:
-    """Address of an optional parameter vector of ``n`` contiguous values."""
-    if t is None:
-        return 0
+def _param(t: torch.Tensor, n: int, device, what: str) -> int:
+    """Address of a parameter vector of ``n`` contiguous values."""
     if t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{what} must be {n} contiguous values")
+        raise ValueError(f"a {what} must be {n} contiguous values")
     if t.device != device:
-        raise ValueError(f"{what} is on {t.device}, the rows on {device}")
+        raise ValueError(f"a {what} is on {t.device}, the rows on {device}")
     return t.data_ptr()
 
 
-def _norm_params(norm: Norm | None, n: int, device, what: str) -> tuple[int, int, int]:
+def _norm_params(norm: Norm | None, n: int, device) -> tuple[int, int, int]:
     """(weight address, bias address, their type) of an optional norm."""
     if norm is None:
         return 0, 0, 0
     weight, bias = norm.weight, norm.bias
+    if weight is None and bias is None:
+        return 0, 0, 0
     _refuse_gradients(weight, bias)
-    code = 0
-    if weight is not None:
-        code = _type(weight.dtype, what)
-        if bias is not None and bias.dtype != weight.dtype:
-            raise ValueError(f"{what} weight and bias differ in type")
-    elif bias is not None:
-        code = _type(bias.dtype, what)
-    return _param(weight, n, device, f"{what} weight"), _param(bias, n, device, f"{what} bias"), code
+    code = _type((bias if weight is None else weight).dtype, "a norm's weight")
+    if weight is None:
+        return 0, _param(bias, n, device, "norm's bias"), code
+    if bias is None:
+        return _param(weight, n, device, "norm's weight"), 0, code
+    if bias.dtype != weight.dtype:
+        raise ValueError("a norm's weight and bias differ in type")
+    return _param(weight, n, device, "norm's weight"), _param(bias, n, device, "norm's bias"), code
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
@@ -241,11 +243,13 @@ def _check_outputs(outs: Sequence[torch.Tensor], inputs: Sequence[torch.Tensor])
 
 def _run(name: str, device: torch.device, *args) -> None:
     """Call an entry point with ``device`` current, on its current stream."""
-    if torch.cuda.current_device() == device.index:
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
-        return
-    with torch.cuda.device(device):
-        _lib.call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() != index:
+        with torch.cuda.device(device):
+            return _run(name, device, *args)
+    rc = getattr(_lib.load(), name)(*args, _lib.raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def rotate_qk(
@@ -307,11 +311,11 @@ def rotate_qk(
         if code == _RMS_ACROSS and max(hq, hk) > (256 if d <= 64 else 128 if d <= 128 else 64):
             raise ValueError(f"too many heads of {d} dims for a norm across heads")
     across = code == _RMS_ACROSS
-    qw, qb, weight_type = _norm_params(query_norm, hq * d if across else d, device, "query norm")
-    kw, kb, k_type = _norm_params(key_norm if key is not None else None, hk * d if across else d, device, "key norm")
-    if (kw or kb) and (qw or qb) and k_type != weight_type:
-        raise ValueError("the norms' weights differ in type")
+    qw, qb, weight_type = _norm_params(query_norm, hq * d if across else d, device)
+    kw, kb, k_type = _norm_params(key_norm if key is not None else None, hk * d if across else d, device)
     if kw or kb:
+        if (qw or qb) and k_type != weight_type:
+            raise ValueError("the norms' weights differ in type")
         weight_type = k_type
 
     address = bits = at = 0
@@ -350,8 +354,12 @@ def rotate_qk(
         raise ValueError("positions and first_token need a rotary")
 
     if out is None:
-        q_out = torch.empty_like(query, dtype=out_dtype)
-        k_out = None if key is None else torch.empty_like(key, dtype=out_dtype)
+        if out_type == in_type:
+            q_out = torch.empty_like(query)
+            k_out = None if key is None else torch.empty_like(key)
+        else:
+            q_out = torch.empty_like(query, dtype=out_dtype)
+            k_out = None if key is None else torch.empty_like(key, dtype=out_dtype)
     else:
         q_out, k_out = out
         pairs = [(q_out, query)] if key is None else [(q_out, query), (k_out, key)]
@@ -383,40 +391,41 @@ def rotate_qk(
     return q_out, k_out
 
 
-def _rows(t: torch.Tensor, like: torch.Tensor, what: str) -> tuple[int, int]:
+def _rows(t: torch.Tensor, shape, device, what: str) -> tuple[int, int]:
     """Element strides (batch, token) of rows ``[batch, tokens, channels]`` or ``[tokens, channels]``."""
-    if t.shape != like.shape:
-        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
-    if t.device != like.device:
-        raise ValueError(f"{what} is on {t.device}, the rows on {like.device}")
+    if t.shape != shape:
+        raise ValueError(f"{what} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the rows on {device}")
     st = t.stride()
-    if st[-1] != 1 and t.shape[-1] > 1:
+    if st[-1] != 1 and shape[-1] > 1:
         raise ValueError(f"{what} needs contiguous channels")
     return (0, st[0]) if len(st) == 2 else (st[0], st[1])
 
 
-def _modulation(t: torch.Tensor | None, like: torch.Tensor, what: str) -> tuple[int, int, int]:
-    """Address and element strides (batch, token; 0 where shared) of a modulation: one vector
-    ``[channels]``, or the rows' dims with size 1 where it is shared."""
+def _modulation(t: torch.Tensor | None, rows, device, what: str) -> tuple[int, int, int]:
+    """Address and element strides (batch, token; 0 where shared) of a modulation of rows of a shape: one
+    vector ``[channels]``, or the rows' dims with size 1 where it is shared."""
     if t is None:
         return 0, 0, 0
-    shape, st, rows = t.shape, t.stride(), like.shape
-    if t.device != like.device:
-        raise ValueError(f"{what} is on {t.device}, the rows on {like.device}")
+    shape, st = t.shape, t.stride()
+    if t.device != device:
+        raise ValueError(f"{what} is on {t.device}, the rows on {device}")
     if shape[-1:] != rows[-1:] or (st[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{what} needs {rows[-1]} contiguous channels")
     if len(shape) == 1:
         return t.data_ptr(), 0, 0
     if len(shape) != len(rows) or any(m != n and m != 1 for m, n in zip(shape, rows)):
         raise ValueError(f"{what} has shape {tuple(shape)}, which does not spread over {tuple(rows)}")
-    steps = [0 if m == 1 else step for m, step in zip(shape, st)]
-    return t.data_ptr(), 0 if len(shape) == 2 else steps[0], steps[-2]
+    token = 0 if shape[-2] == 1 else st[-2]
+    return t.data_ptr(), 0 if len(shape) == 2 or shape[0] == 1 else st[0], token
 
 
 def _norm_rows(what: str, x, branch, gate, branch_norm, norm, scale, shift, x_out, h, h_dtype):
-    if x.dim() not in (2, 3):
+    shape = x.shape
+    if len(shape) not in (2, 3):
         raise ValueError("rows are [batch, tokens, channels] or [tokens, channels]")
-    c = x.shape[-1]
+    c = shape[-1]
     if c % 8 or not 8 <= c <= 16384:
         raise ValueError("channels must be a multiple of 8 up to 16384")
     device = x.device
@@ -424,58 +433,76 @@ def _norm_rows(what: str, x, branch, gate, branch_norm, norm, scale, shift, x_ou
     if h_type != x_type and x_type != 2:
         raise ValueError("only float32 rows have a norm or a branch of another type")
     _refuse_gradients(x, branch, gate, scale, shift)
-    xs = _rows(x, x, "rows")
-    bs = (0, 0) if branch is None else _rows(branch, x, "branch")
-    mods = [t for t in (scale, shift, gate) if t is not None]
-    mod_type = _type(mods[0].dtype, "modulations") if mods else 0
-    if any(t.dtype != mods[0].dtype for t in mods):
-        raise ValueError("scale, shift and gate differ in type")
-    sc, sh, ga = (_modulation(t, x, n) for t, n in ((scale, "scale"), (shift, "shift"), (gate, "gate")))
-    for n in (norm, branch_norm):
-        if n is not None and n.across_heads:
-            raise ValueError("a norm across heads belongs to rotate_qk")
-    w, wb, w_type = _norm_params(norm, c, device, "norm")
-    bw, bb, b_type = _norm_params(branch_norm, c, device, "branch norm")
-    outs, ins = [], []
+    xs = _rows(x, shape, device, "rows")
+    bs = (0, 0) if branch is None else _rows(branch, shape, device, "branch")
+    mod_dtype = None
+    for t in (scale, shift, gate):
+        if t is not None:
+            if mod_dtype is not None and t.dtype != mod_dtype:
+                raise ValueError("scale, shift and gate differ in type")
+            mod_dtype = t.dtype
+    mod_type = 0 if mod_dtype is None else _type(mod_dtype, "modulations")
+    sc = _modulation(scale, shape, device, "scale")
+    sh = _modulation(shift, shape, device, "shift")
+    ga = _modulation(gate, shape, device, "gate")
+    norm_code = branch_code = 0
+    eps = branch_eps = 0.0
+    if norm is not None:
+        norm_code, eps = norm.code, norm.eps
+    if branch_norm is not None:
+        branch_code, branch_eps = branch_norm.code, branch_norm.eps
+    if norm_code == _RMS_ACROSS or branch_code == _RMS_ACROSS:
+        raise ValueError("a norm across heads belongs to rotate_qk")
+    w, wb, w_type = _norm_params(norm, c, device)
+    bw, bb, b_type = _norm_params(branch_norm, c, device)
+    if x_out is not None or h is not None:
+        _check_row_outputs(x, branch, (scale, shift, gate), norm, x_out, h, h_dtype)
+    b_ptr = xo_ptr = h_ptr = 0
     xos = hs = (0, 0)
     if branch is not None:
         if x_out is None:
             x_out = torch.empty_like(x)
-        else:
-            outs.append(x_out)
-            ins.append(x)
-            if x_out.dtype != x.dtype:
-                raise ValueError("the sum has the residual's dtype")
-        xos = _rows(x_out, x, "out")
+        xos = _rows(x_out, shape, device, "out")
+        b_ptr, xo_ptr = branch.data_ptr(), x_out.data_ptr()
     if norm is not None:
         if h is None:
-            h = torch.empty_like(x if branch is None else branch, dtype=h_dtype)
-        else:
-            outs.append(h)
-            ins.append(x if branch is None else branch)
-            if h.dtype != h_dtype:
-                raise ValueError("the norm's out differs in dtype")
-        hs = _rows(h, x, "out")
-    if outs:
-        every = [t for t in (x, branch) if t is not None]
-        _check_outputs(outs, ins)
-        for o, mine in zip(outs, ins):
-            for t in every + [t for t in (scale, shift, gate) if t is not None]:
-                if t is not mine and not _apart(o, t):
-                    raise ValueError("an output overlaps an input (it may only be that input itself)")
+            like = x if branch is None else branch
+            h = torch.empty_like(like) if like.dtype == h_dtype else torch.empty_like(like, dtype=h_dtype)
+        hs = _rows(h, shape, device, "out")
+        h_ptr = h.data_ptr()
     if not x.is_cuda:
         raise ValueError(f"{what} runs on CUDA tensors only")
-    b, s = (1, x.shape[0]) if x.dim() == 2 else (x.shape[0], x.shape[1])
+    b, s = (1, shape[0]) if len(shape) == 2 else (shape[0], shape[1])
     if b == 0 or s == 0:
         return x_out, h
-    args = _NORM_ARGS.pack(
-        x.data_ptr(), 0 if branch is None else branch.data_ptr(), 0 if branch is None else x_out.data_ptr(),
-        0 if norm is None else h.data_ptr(), *xs, *bs, *xos, *hs, sc[0], sh[0], ga[0], *sc[1:], *sh[1:], *ga[1:], w, wb,
-        bw, bb, b, s, c, x_type, h_type, 0 if norm is None else norm.code,
-        0 if branch_norm is None else branch_norm.code, w_type, b_type, mod_type, 0.0 if norm is None else norm.eps,
-        0.0 if branch_norm is None else branch_norm.eps)
-    _run("recap_norm_rows", device, args)
+    _run("recap_norm_rows", device, _NORM_ARGS.pack(
+        x.data_ptr(), b_ptr, xo_ptr, h_ptr, *xs, *bs, *xos, *hs, sc[0], sh[0], ga[0], sc[1], sc[2], sh[1], sh[2], ga[1],
+        ga[2], w, wb, bw, bb, b, s, c, x_type, h_type, norm_code, branch_code, w_type, b_type, mod_type, eps,
+        branch_eps))
     return x_out, h
+
+
+def _check_row_outputs(x, branch, mods, norm, x_out, h, h_dtype) -> None:
+    """Given outputs: of the right type, each its own input of the same kind or apart from every input."""
+    outs, own = [], []
+    if x_out is not None:
+        if x_out.dtype != x.dtype:
+            raise ValueError("the sum has the residual's dtype")
+        outs.append(x_out)
+        own.append(x)
+    if h is not None:
+        if h.dtype != h_dtype:
+            raise ValueError("the norm's out differs in dtype")
+        outs.append(h)
+        own.append(x if branch is None else branch)
+    for o in outs:
+        if o.shape != x.shape or o.device != x.device:
+            raise ValueError("out must have the rows' shape and device")
+    _check_outputs(outs, own)
+    for o, mine in zip(outs, own):
+        for t in (x, branch, *mods):
+            if t is not None and t is not mine and not _apart(o, t):
+                raise ValueError("an output overlaps an input (it may only be that input itself)")
 
 
 def modulated_norm(

@@ -40,6 +40,20 @@ struct Raw8 {
 __device__ __forceinline__ uint4 ld_v4(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ uint2 ld_v2(const void* p) { return *reinterpret_cast<const uint2*>(p); }
 
+// Asynchronous copies from global to shared memory, in groups that the issuing thread waits for.
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy8(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last n committed groups of this thread have landed.
+template <int n>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+
 // Values p[0 .. 8).
 template <typename T>
 __device__ __forceinline__ void load8(Raw8<T>& r, const T* p) {
@@ -60,6 +74,17 @@ __device__ __forceinline__ void load4x2(Raw8<T>& r, const T* p, const T* q) {
   } else {
     const uint2 a = ld_v2(p), b = ld_v2(q);
     r.w[0] = a.x, r.w[1] = a.y, r.w[2] = b.x, r.w[3] = b.y;
+  }
+}
+// Values p[0 .. 4) as the first four.
+template <typename T>
+__device__ __forceinline__ void load4(Raw8<T>& r, const T* p) {
+  if constexpr (sizeof(T) == 4) {
+    const uint4 a = ld_v4(p);
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+  } else {
+    const uint2 a = ld_v2(p);
+    r.w[0] = a.x, r.w[1] = a.y;
   }
 }
 template <typename T>
@@ -87,6 +112,13 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {
   }
 }
 template <typename T>
+__device__ __forceinline__ void store4(T* p, const float (&x)[8]) {
+  if constexpr (sizeof(T) == 4)
+    *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+  else
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]));
+}
+template <typename T>
 __device__ __forceinline__ void store4x2(T* p, T* q, const float (&x)[8]) {
   if constexpr (sizeof(T) == 4) {
     *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
@@ -97,34 +129,71 @@ __device__ __forceinline__ void store4x2(T* p, T* q, const float (&x)[8]) {
   }
 }
 
-// Values p[at .. at + n) of a small parameter vector whose type is known at run time (norm
-// weights and biases, modulations): n is 4 or 8, the address aligned to n values.
-template <int N>
-__device__ __forceinline__ void load_param(float* x, const void* p, int64_t at, int type) {
+template <typename T>
+__device__ __forceinline__ void zero8(Raw8<T>& r) {
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(2 * sizeof(T)); ++i) r.w[i] = 0;
+}
+
+// Eight values at p[at] of a parameter vector whose type is known at run time (norm weights
+// and biases, modulations), as loaded and widened; the address is aligned to 16 bytes.
+struct RawParam8 {
+  uint32_t w[8];
+};
+// kSplit: two runs of four values at at0 and at1, else eight values at at0.
+template <bool kSplit>
+__device__ __forceinline__ void load_param_raw(RawParam8& r, const void* p, int64_t at0, int64_t at1, int type) {
   if (type == kTypeF32) {
-    const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const float4 v = s[i];
-      x[4 * i] = v.x, x[4 * i + 1] = v.y, x[4 * i + 2] = v.z, x[4 * i + 3] = v.w;
-    }
-    return;
-  }
-  uint32_t w[N / 2];
-  const uint16_t* s = static_cast<const uint16_t*>(p) + at;
-  if constexpr (N == 8) {
-    const uint4 v = ld_v4(s);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    const float* f = static_cast<const float*>(p);
+    const uint4 a = ld_v4(f + at0), b = ld_v4(f + (kSplit ? at1 : at0 + 4));
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w, r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+  } else if (kSplit) {
+    const uint16_t* h = static_cast<const uint16_t*>(p);
+    const uint2 a = ld_v2(h + at0), b = ld_v2(h + at1);
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = b.x, r.w[3] = b.y;
   } else {
-    const uint2 v = ld_v2(s);
-    w[0] = v.x, w[1] = v.y;
+    const uint4 a = ld_v4(static_cast<const uint16_t*>(p) + at0);
+    r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
   }
+}
+__device__ __forceinline__ void widen_param8(float (&x)[8], const RawParam8& r, int type) {
+  if (type == kTypeF32) {
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) {
-    const float2 f = type == kTypeBf16 ? unpack2<__nv_bfloat16>(w[i]) : unpack2<__half>(w[i]);
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+    for (int i = 0; i < 8; ++i) x[i] = __uint_as_float(r.w[i]);
+  } else if (type == kTypeBf16) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<__nv_bfloat16>(r.w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<__half>(r.w[i]);
+      x[2 * i] = f.x, x[2 * i + 1] = f.y;
+    }
   }
+}
+// Eight values of kBytes (2 or 4) each at a byte address, as loaded.
+template <bool kSplit, int kBytes>
+__device__ __forceinline__ void load_own(uint32_t (&w)[2 * kBytes], const void* row, int c0, int c1) {
+  const char* p = static_cast<const char*>(row);
+  if constexpr (kBytes == 4) {
+    const uint4 a = ld_v4(p + c0 * 4), b = ld_v4(p + c1 * 4);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w, w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+  } else if constexpr (kSplit) {
+    const uint2 a = ld_v2(p + c0 * 2), b = ld_v2(p + c1 * 2);
+    w[0] = a.x, w[1] = a.y, w[2] = b.x, w[3] = b.y;
+  } else {
+    const uint4 a = ld_v4(p + c0 * 2);
+    w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+  }
+}
+template <bool kSplit>
+__device__ __forceinline__ void load_param(float (&x)[8], const void* p, int64_t at0, int64_t at1, int type) {
+  RawParam8 r;
+  load_param_raw<kSplit>(r, p, at0, at1, type);
+  widen_param8(x, r, type);
 }
 
 // Sum over aligned groups of N lanes, in every lane.

@@ -244,6 +244,12 @@ enum : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2, kNormRmsAcross = 3 };
 constexpr int kMaxAxes = 4;
 constexpr int kMaxPairs = 128;
 
+// Division by a number fixed for a launch: n mul >> shift, for n < 2^31.
+struct Divisor {
+  uint32_t mul;
+  int shift;
+};
+
 struct RotateArgs {
   const void* x[2];                     // q, k [batch, heads, S, D], D contiguous
   void* out[2];
@@ -260,7 +266,10 @@ struct RotateArgs {
   int64_t first_token, video_offset, video_tokens;  // the grid starts at token video_offset
   int axes, pairs, halves;
   int grid[kMaxAxes];
-  int split_log2[2], token_fast[2];     // set by launch_rotate
+  // set by launch_rotate: batch * S, divisors by S and the grid's sizes, groups of a token, their order
+  uint32_t tokens;
+  Divisor s_div, grid_div[kMaxAxes];
+  int split_log2, token_fast;
   uint64_t turns[kMaxPairs];            // turns of the pair per position, times 2^64
   uint64_t phase[kMaxPairs];
   uint8_t axis[kMaxPairs];
@@ -279,8 +288,9 @@ struct NormArgs {
   const void *weight, *bias, *branch_weight, *branch_bias;  // [C] (nullable each)
   float eps, branch_eps;
   int batch, S, C, x_type, h_type, norm, branch_norm, weight_type, branch_weight_type, mod_type;
+  int blocks;                           // of a sample, set by launch_norm_rows
 };
 int norm_max_channels();
-int launch_norm_rows(const NormArgs& a, cudaStream_t s);
+int launch_norm_rows(NormArgs& a, cudaStream_t s);
 
 }  // namespace recap

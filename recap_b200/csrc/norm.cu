@@ -7,10 +7,12 @@
 // vectors of C values that a batch shares, or one of its samples, or that belong to one token.
 //
 // Bound by memory: every row is read once and written once and lies in registers between.  A
-// row lies on one block of W warps, kVec times eight values per thread; the sums go over lanes
-// and then over the warps through shared memory.  Modulations that many rows share come from
-// L1 and L2 after the first.  h is formed from the fp32 x', not from its rounded copy: one
-// rounding instead of two.
+// row lies on one block, kVec times eight values per thread; a block takes kRows tokens of a
+// sample at once, so that their loads are in flight together, their sums share shuffles and
+// barriers, and modulations that tokens share are read once for them.  Modulations of single
+// tokens are loaded with the rows, ahead of the sums.  fp32 rows are read in runs of four values,
+// the next lane's run following: 16 bytes a lane side by side.  h is formed from the fp32 x',
+// not from its rounded copy: one rounding instead of two.
 #include "elements.cuh"
 
 namespace recap {
@@ -19,175 +21,353 @@ namespace {
 constexpr int kMaxVec = 4;     // vectors of eight values a thread holds of a row
 constexpr int kMaxWarps = 16;  // warps of a row
 
-// Sum over the block, in every thread.  `buf` holds one float per warp; two calls in a row use
-// different buffers, so that one barrier each is enough.
-__device__ __forceinline__ float block_sum(float v, float* buf, int warps) {
-  v = lanes_sum<32>(v);
-  if (warps == 1) return v;
-  if ((threadIdx.x & 31) == 0) buf[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float s = 0.f;
-  for (int i = 0; i < warps; ++i) s += buf[i];
-  return s;
+// Sums of kRows (1, 2, 4) values over the warp.  Two values share the steps of one: each half of
+// the lanes keeps one value and hands the other over, then goes on with its own.  On return
+// v[0] of lane l is the sum of value l / (32 / kRows).
+template <int kRows>
+__device__ __forceinline__ float warp_sums(float (&v)[kRows]) {
+  const int lane = threadIdx.x & 31;
+  if constexpr (kRows == 4) {
+    const bool up = lane & 16;
+    const float k0 = up ? v[2] : v[0], k1 = up ? v[3] : v[1];
+    const float o0 = up ? v[0] : v[2], o1 = up ? v[1] : v[3];
+    v[0] = k0 + __shfl_xor_sync(0xffffffffu, o0, 16);
+    v[1] = k1 + __shfl_xor_sync(0xffffffffu, o1, 16);
+  }
+  if constexpr (kRows >= 2) {
+    constexpr int o = kRows == 4 ? 8 : 16;
+    const bool up = lane & o;
+    const float keep = up ? v[1] : v[0], other = up ? v[0] : v[1];
+    v[0] = keep + __shfl_xor_sync(0xffffffffu, other, o);
+  }
+  return lanes_sum<32 / kRows>(v[0]);
+}
+
+// Sums of kRows values over the block, in every thread.  `buf` holds kRows * kMaxWarps floats; calls
+// take two buffers in turn, so that one barrier each is enough: a buffer is written again only after
+// the next call's barrier, which every thread reaches after it has read it.
+template <int kRows>
+__device__ __forceinline__ void block_sum(float (&v)[kRows], float* buf, int warps) {
+  constexpr int kPer = 32 / kRows;  // lanes of a value
+  constexpr int kUse = kPer < kMaxWarps ? kPer : kMaxWarps;
+  const int lane = threadIdx.x & 31;
+  float s = warp_sums<kRows>(v);
+  if (warps > 1) {
+    if (lane % kPer == 0) buf[(lane / kPer) * kMaxWarps + (threadIdx.x >> 5)] = s;
+    __syncthreads();
+    const float* mine = buf + (lane / kPer) * kMaxWarps;
+    s = 0.f;
+#pragma unroll
+    for (int w = 0; w < kMaxWarps; w += kUse) {
+      const int at = w + lane % kUse;
+      if (at < warps) s += mine[at];
+    }
+    s = lanes_sum<kUse>(s);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) v[r] = kRows == 1 ? s : __shfl_sync(0xffffffffu, s, r * kPer);
+}
+
+// The columns of a thread's vector v: two runs of four values, apart (kSplit) or one after the other.
+template <bool kSplit>
+struct Columns {
+  int c0, c1;
+  bool in0, in1;
+  __device__ __forceinline__ Columns(int v, int C) {
+    if (kSplit) {
+      c0 = (2 * v * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 4;
+      c1 = c0 + 4 * static_cast<int>(blockDim.x);
+      in0 = c0 < C;
+      in1 = c1 < C;
+    } else {
+      c0 = (v * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
+      c1 = c0 + 4;
+      in0 = in1 = c0 < C;
+    }
+  }
+};
+
+// A row's values of those columns, zero past its end.
+template <bool kSplit, typename T>
+__device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Columns<kSplit>& c, bool live) {
+  if (live && c.in1) {
+    if constexpr (kSplit)
+      load4x2(r, row + c.c0, row + c.c1);
+    else
+      load8(r, row + c.c0);
+  } else {
+    zero8(r);
+    if (kSplit && live && c.in0) load4(r, row + c.c0);
+  }
+}
+template <bool kSplit, typename T>
+__device__ __forceinline__ void store_columns(T* row, const Columns<kSplit>& c, const float (&x)[8]) {
+  if (c.in1) {
+    if constexpr (kSplit)
+      store4x2(row + c.c0, row + c.c1, x);
+    else
+      store8(row + c.c0, x);
+  } else if (kSplit && c.in0) {
+    store4(row + c.c0, x);
+  }
 }
 
 // norm(x) in place: the row mean (layer norm), then the mean square, in two sums.
-template <int kVec>
-__device__ __forceinline__ void norm_rows(float (&x)[kVec][8], int layer, int C, float eps, float* buf, int warps) {
+template <int kRows, int kVec, bool kSplit>
+__device__ __forceinline__ void norm_rows(float (&x)[kRows][kVec][8], int layer, int C, float eps, float* buf,
+                                          int& turn, int warps) {
   const float inv = 1.f / static_cast<float>(C);
+  float t[kRows];
   if (layer) {
-    float m = 0.f;
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+      for (int v = 0; v < kVec; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) add2(m0, m1, x[r][v][j], x[r][v][j + 1]);
+      t[r] = m0 + m1;
+    }
+    block_sum(t, buf + (turn ^= kRows * kMaxWarps), warps);
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+      const Columns<kSplit> c(v, C);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const float m = -t[r] * inv;
+        const float m0 = c.in0 ? m : 0.f, m1 = c.in1 ? m : 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          add2(x[r][v][j], x[r][v][j + 1], m0, m0);
+          add2(x[r][v][j + 4], x[r][v][j + 5], m1, m1);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    float s0 = 0.f, s1 = 0.f;
 #pragma unroll
     for (int v = 0; v < kVec; ++v)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) m += x[v][j];
-    m = block_sum(m, buf, warps) * inv;
-#pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-      const bool in = (v * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8 < C;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[v][j] = in ? x[v][j] - m : 0.f;
-    }
+      for (int j = 0; j < 8; j += 2)
+        fma2(s0, s1, x[r][v][j], x[r][v][j + 1], x[r][v][j], x[r][v][j + 1], s0, s1);
+    t[r] = s0 + s1;
   }
-  float ss = 0.f;
+  block_sum(t, buf + (turn ^= kRows * kMaxWarps), warps);
 #pragma unroll
-  for (int v = 0; v < kVec; ++v)
+  for (int r = 0; r < kRows; ++r) {
+    const float q = rsqrtf(fmaf(t[r], inv, eps));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(x[v][j], x[v][j], ss);
-  const float r = rsqrtf(block_sum(ss, buf + kMaxWarps, warps) * inv + eps);
+    for (int v = 0; v < kVec; ++v)
 #pragma unroll
-  for (int v = 0; v < kVec; ++v)
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[v][j] *= r;
-}
-
-// x = x * weight + bias with weight and bias optional parameter vectors
-__device__ __forceinline__ void affine8(float (&x)[8], const void* w, const void* b, int64_t at, int type) {
-  float p[8];
-  if (w != nullptr) {
-    load_param<8>(p, w, at, type);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] *= p[j];
-  }
-  if (b != nullptr) {
-    load_param<8>(p, b, at, type);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] += p[j];
+      for (int j = 0; j < 8; j += 2) mul2(x[r][v][j], x[r][v][j + 1], q, q);
   }
 }
 
-// Values [at, at + 8) of modulation m (0 scale, 1 shift, 2 gate) for sample b, token s.
-__device__ __forceinline__ void modulation8(float (&p)[8], const NormArgs& a, int m, int b, int s, int at) {
-  load_param<8>(p, a.mod[m], b * a.mod_stride[m][0] + s * a.mod_stride[m][1] + at, a.mod_type);
+// x = x * p or x + p, eight values
+__device__ __forceinline__ void mul8(float (&x)[8], const float (&p)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) mul2(x[j], x[j + 1], p[j], p[j + 1]);
+}
+__device__ __forceinline__ void add8(float (&x)[8], const float (&p)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) add2(x[j], x[j + 1], p[j], p[j + 1]);
 }
 
-template <typename TX, typename TH, int kVec, bool kGate>
-__global__ void __launch_bounds__(kMaxWarps * 32) norm_kernel(const __grid_constant__ NormArgs a) {
-  __shared__ float buf[4 * kMaxWarps];
+// How a block comes by its modulations: read when needed, one vector for its tokens (or its one
+// token); or each token's own, of 16 or 32 bits a value, loaded with the rows.
+enum : int { kModsLate = 0, kMods16 = 2, kMods32 = 4 };
+
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods>
+__global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm_kernel(const __grid_constant__ NormArgs a) {
+  constexpr bool kSplit = sizeof(TX) == 4;
+  constexpr bool kOwn = kMods != kModsLate;
+  __shared__ float buf[2 * kRows * kMaxWarps];
+  int turn = 0;
   const int warps = blockDim.x >> 5;
-  const int b = blockIdx.x / a.S;
-  const int s = blockIdx.x - b * a.S;
   const int C = a.C;
-  const TX* xr = static_cast<const TX*>(a.x) + b * a.x_stride[0] + s * a.x_stride[1];
-  float x[kVec][8];
-  Raw8<TX> rx[kVec];
-  Raw8<TH> ry[kGate ? kVec : 1];
+  const int b = a.batch == 1 ? 0 : blockIdx.x / a.blocks;
+  const int s0 = (blockIdx.x - b * a.blocks) * kRows;
+  const int rows = kRows == 1 ? 1 : min(kRows, a.S - s0);
+
+  Raw8<TX> rx[kRows][kVec];
+  Raw8<TH> ry[kGate ? kRows : 1][kVec];
+  {
+    const TX* xr = static_cast<const TX*>(a.x) + b * a.x_stride[0] + s0 * a.x_stride[1];
+    const TH* yr = nullptr;
+    if constexpr (kGate) yr = static_cast<const TH*>(a.branch) + b * a.branch_stride[0] + s0 * a.branch_stride[1];
 #pragma unroll
-  for (int v = 0; v < kVec; ++v) {
-    const int at = (v * blockDim.x + threadIdx.x) * 8;
-    if (at < C) {
-      load8(rx[v], xr + at);
-      if constexpr (kGate)
-        load8(ry[v], static_cast<const TH*>(a.branch) + b * a.branch_stride[0] + s * a.branch_stride[1] + at);
+    for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) {
+        const Columns<kSplit> c(v, C);
+        load_columns<kSplit>(rx[r][v], xr, c, r < rows);
+        if constexpr (kGate) load_columns<kSplit>(ry[r][v], yr, c, r < rows);
+      }
+      xr += a.x_stride[1];
+      if constexpr (kGate) yr += a.branch_stride[1];
     }
   }
+  // modulations of single tokens are as far away as the rows: ask for them now
+  uint32_t own[kOwn ? 3 : 1][kOwn ? kRows : 1][kOwn ? kVec : 1][kOwn ? 2 * kMods : 1];
+  if constexpr (kOwn) {
+#pragma unroll
+    for (int m = 0; m < (kGate ? 3 : 2); ++m) {
+      if (a.mod[m] == nullptr) continue;
+      const char* row = static_cast<const char*>(a.mod[m]) + (b * a.mod_stride[m][0] + s0 * a.mod_stride[m][1]) * kMods;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+          const Columns<kSplit> c(v, C);
+          if (r < rows && c.in0) load_own<kSplit, kMods>(own[m][r][v], row, c.c0, c.in1 ? c.c1 : c.c0);
+        }
+        row += a.mod_stride[m][1] * kMods;
+      }
+    }
+  }
+  // modulation m of the block's row r; late ones are read for the first row and stay
+  auto modulation = [&](float (&p)[8], int m, int r, int v, int c0, int c1) {
+    if constexpr (kOwn) {
+      RawParam8 w;
+#pragma unroll
+      for (int j = 0; j < 2 * kMods; ++j) w.w[j] = own[m][r][v][j];
+      widen_param8(p, w, kMods == kMods32 ? kTypeF32 : a.mod_type);
+    } else if (r == 0) {
+      const int64_t at = b * a.mod_stride[m][0] + (kRows == 1 ? s0 * a.mod_stride[m][1] : 0);
+      load_param<kSplit>(p, a.mod[m], at + c0, at + c1, a.mod_type);
+    }
+  };
+
+  float x[kRows][kVec][8];
+  float p[8];
   if constexpr (kGate) {
 #pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int v = 0; v < kVec; ++v) widen8(x[r][v], ry[r][v]);
+    if (a.branch_norm != kNormNone)
+      norm_rows<kRows, kVec, kSplit>(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, turn, warps);
+    TX* out = static_cast<TX*>(a.x_out) + b * a.x_out_stride[0] + s0 * a.x_out_stride[1];
+#pragma unroll
     for (int v = 0; v < kVec; ++v) {
+      const Columns<kSplit> c(v, C);
+      if (!c.in0) continue;
+      const int c1 = c.in1 ? c.c1 : c.c0;  // a run past the row reads the one before it and is not stored
+      if (a.branch_weight != nullptr) {
+        load_param<kSplit>(p, a.branch_weight, c.c0, c1, a.branch_weight_type);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[v][j] = 0.f;
-      if (static_cast<int>(v * blockDim.x + threadIdx.x) * 8 < C) widen8(x[v], ry[v]);
-    }
-    if (a.branch_norm != kNormNone) norm_rows(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, warps);
+        for (int r = 0; r < kRows; ++r) mul8(x[r][v], p);
+      }
+      if (a.branch_bias != nullptr) {
+        load_param<kSplit>(p, a.branch_bias, c.c0, c1, a.branch_weight_type);
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) {
-      const int at = (v * blockDim.x + threadIdx.x) * 8;
-      if (at < C) {
-        affine8(x[v], a.branch_weight, a.branch_bias, at, a.branch_weight_type);
-        float p[8];
-        if (a.mod[2] != nullptr) {
-          modulation8(p, a, 2, b, s, at);
+        for (int r = 0; r < kRows; ++r) add8(x[r][v], p);
+      }
+      if (a.mod[2] != nullptr) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) x[v][j] *= p[j];
+        for (int r = 0; r < kRows; ++r) {
+          modulation(p, 2, r, v, c.c0, c1);
+          mul8(x[r][v], p);
         }
-        widen8(p, rx[v]);
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[v][j] += p[j];
-        store8(static_cast<TX*>(a.x_out) + b * a.x_out_stride[0] + s * a.x_out_stride[1] + at, x[v]);
+      for (int r = 0; r < kRows; ++r) {
+        float res[8];
+        widen8(res, rx[r][v]);
+        add8(x[r][v], res);
+        if (r < rows) store_columns<kSplit>(out + r * a.x_out_stride[1], c, x[r][v]);
+        if (kSplit && !c.in1) x[r][v][4] = x[r][v][5] = x[r][v][6] = x[r][v][7] = 0.f;  // out of the sums
       }
     }
     if (a.norm == kNormNone) return;
   } else {
 #pragma unroll
-    for (int v = 0; v < kVec; ++v) {
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[v][j] = 0.f;
-      if (static_cast<int>(v * blockDim.x + threadIdx.x) * 8 < C) widen8(x[v], rx[v]);
-    }
+      for (int v = 0; v < kVec; ++v) widen8(x[r][v], rx[r][v]);
   }
-  norm_rows(x, a.norm == kNormLayer, C, a.eps, buf + 2 * kMaxWarps, warps);
+  norm_rows<kRows, kVec, kSplit>(x, a.norm == kNormLayer, C, a.eps, buf, turn, warps);
+  TH* out = static_cast<TH*>(a.h) + b * a.h_stride[0] + s0 * a.h_stride[1];
 #pragma unroll
   for (int v = 0; v < kVec; ++v) {
-    const int at = (v * blockDim.x + threadIdx.x) * 8;
-    if (at < C) {
-      affine8(x[v], a.weight, a.bias, at, a.weight_type);
-      float p[8];
-      if (a.mod[0] != nullptr) {
-        modulation8(p, a, 0, b, s, at);
+    const Columns<kSplit> c(v, C);
+    if (!c.in0) continue;
+    const int c1 = c.in1 ? c.c1 : c.c0;
+    if (a.weight != nullptr) {
+      load_param<kSplit>(p, a.weight, c.c0, c1, a.weight_type);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[v][j] = fmaf(x[v][j], p[j], x[v][j]);
-      }
-      if (a.mod[1] != nullptr) {
-        modulation8(p, a, 1, b, s, at);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[v][j] += p[j];
-      }
-      store8(static_cast<TH*>(a.h) + b * a.h_stride[0] + s * a.h_stride[1] + at, x[v]);
+      for (int r = 0; r < kRows; ++r) mul8(x[r][v], p);
     }
+    if (a.bias != nullptr) {
+      load_param<kSplit>(p, a.bias, c.c0, c1, a.weight_type);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) add8(x[r][v], p);
+    }
+    if (a.mod[0] != nullptr) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        modulation(p, 0, r, v, c.c0, c1);
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+          fma2(x[r][v][j], x[r][v][j + 1], x[r][v][j], x[r][v][j + 1], p[j], p[j + 1], x[r][v][j], x[r][v][j + 1]);
+      }
+    }
+    if (a.mod[1] != nullptr) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        modulation(p, 1, r, v, c.c0, c1);
+        add8(x[r][v], p);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (r < rows) store_columns<kSplit>(out + r * a.h_stride[1], c, x[r][v]);
   }
 }
 
-
-
-template <typename TX, typename TH, int kVec>
-int launch_gate(const NormArgs& a, int threads, cudaStream_t s) {
-  const unsigned rows = static_cast<unsigned>(static_cast<int64_t>(a.batch) * a.S);
+template <typename TX, typename TH, int kVec, int kRows, int kMods>
+int launch_gate(NormArgs& a, int threads, cudaStream_t s) {
+  a.blocks = (a.S + kRows - 1) / kRows;
+  const unsigned blocks = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.blocks);
   if (a.branch != nullptr)
-    norm_kernel<TX, TH, kVec, true><<<rows, threads, 0, s>>>(a);
+    norm_kernel<TX, TH, kVec, kRows, true, kMods><<<blocks, threads, 0, s>>>(a);
   else
-    norm_kernel<TX, TH, kVec, false><<<rows, threads, 0, s>>>(a);
+    norm_kernel<TX, TH, kVec, kRows, false, kMods><<<blocks, threads, 0, s>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
 template <typename TX, typename TH>
-int launch_vec(const NormArgs& a, cudaStream_t s) {
-  // the fewest warps that hold a row at kMaxVec vectors a thread, then the fewest vectors
+int launch_vec(NormArgs& a, cudaStream_t s) {
+  // few values a thread, so that a block of up to 384 threads keeps four tokens in registers and two
+  // such blocks fit an SM; longer rows take more values a thread and fewer tokens
   const int vecs = a.C / 8;
-  int warps = 1;
-  while (warps * 32 * kMaxVec < vecs) warps *= 2;
-  const int per = (vecs + warps * 32 - 1) / (warps * 32);
-  const int threads = warps * 32;
-  if (per == 1) return launch_gate<TX, TH, 1>(a, threads, s);
-  if (per == 2) return launch_gate<TX, TH, 2>(a, threads, s);
-  if (per == 3) return launch_gate<TX, TH, 3>(a, threads, s);
-  return launch_gate<TX, TH, 4>(a, threads, s);
+  const int per = vecs <= 384 ? 1 : vecs <= 768 ? 2 : 4;
+  const int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
+  bool shared = true;
+  for (int m = 0; m < 3; ++m) shared = shared && (a.mod[m] == nullptr || a.mod_stride[m][1] == 0);
+  const bool narrow = a.mod_type != kTypeF32;
+  // tokens by the block only where blocks of one token would be more than the device holds
+  const bool many = static_cast<int64_t>(a.batch) * a.S >= 2048;
+  if (per == 1) {
+    if (shared) return many ? launch_gate<TX, TH, 1, 4, kModsLate>(a, threads, s) : launch_gate<TX, TH, 1, 1, kModsLate>(a, threads, s);
+    if (!narrow) return launch_gate<TX, TH, 1, 1, kMods32>(a, threads, s);
+    return many ? launch_gate<TX, TH, 1, 2, kMods16>(a, threads, s) : launch_gate<TX, TH, 1, 1, kMods16>(a, threads, s);
+  }
+  if (per == 2) {
+    if (shared && many) return launch_gate<TX, TH, 2, 2, kModsLate>(a, threads, s);
+    if (!shared && narrow) return launch_gate<TX, TH, 2, 1, kMods16>(a, threads, s);
+    return launch_gate<TX, TH, 2, 1, kModsLate>(a, threads, s);
+  }
+  return launch_gate<TX, TH, 4, 1, kModsLate>(a, threads, s);
 }
 
 }  // namespace
 
 int norm_max_channels() { return kMaxWarps * 32 * kMaxVec * 8; }
 
-int launch_norm_rows(const NormArgs& a, cudaStream_t s) {
+int launch_norm_rows(NormArgs& a, cudaStream_t s) {
   if (a.x_type == kTypeBf16 && a.h_type == kTypeBf16) return launch_vec<__nv_bfloat16, __nv_bfloat16>(a, s);
   if (a.x_type == kTypeF16 && a.h_type == kTypeF16) return launch_vec<__half, __half>(a, s);
   if (a.x_type == kTypeF32 && a.h_type == kTypeF32) return launch_vec<float, float>(a, s);

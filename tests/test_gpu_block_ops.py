@@ -10,8 +10,10 @@ Tolerances count roundings, u = 2^-24 of fp32 and eps(t) of the output type:
   channels: 32 in the thread, 5 lanes, 16 warps), the mean taken off adds one, the mean square is off by
   (k + 2) u relatively and by 2 u M sqrt(n) through the rounded differences, of which the root
   halves the former; rsqrt 2 u, the products with weight and bias 3 u, scale and shift 3 u, the turn 3 u for
-  its products and sums and 3 u for sine and cosine (2 ulp and 2^-25 of half a turn).
-  Added up: (13 + 1 + 8 + 2 + 3 + 6) = 33, + 2 sqrt(256) = 65 u for ``rotate_qk`` within one head,
+  its products and sums and 4 u for sine and cosine (2 ulp of sincospif, and 2^-25 of half a turn from
+  the angle's rounding), or 15 u where the output has 16 bits (__sincosf on [-pi, pi]: 2^-21.19, under 8 u;
+  the angle in radians off by 2^-25 pi from its turns and 2^-24 pi / 2 from the product, under 4 u; the rest is slack).
+  Added up: (13 + 1 + 8 + 2 + 3) = 27, + 2 sqrt(256), + 7 or 18 u for ``rotate_qk`` within one head,
   and 53 + 1 + 28 + 2 + 3 + 3 = 90, + 2 sqrt(n), for the rows."""
 
 import math
@@ -62,8 +64,9 @@ def ref_norm64(x, norm, dims):
     return y, big.expand_as(y)
 
 
-def ref_rotate64(x, norm, rotary, positions, first_token=0):
+def ref_rotate64(x, norm, rotary, positions, first_token=0, out_dtype=None):
     """64-bit reference of one tensor [b, h, s, d]: (result, fp32 error bound)."""
+    turn = 3 + (4 if (out_dtype or x.dtype) == F32 else 15)
     x = x.double()
     y, big = ref_norm64(x, norm, (1, 3) if norm is not None and norm.across_heads else (3,))
     n = x.shape[1] * x.shape[3] if norm is not None and norm.across_heads else x.shape[3]
@@ -99,7 +102,7 @@ def ref_rotate64(x, norm, rotary, positions, first_token=0):
     y0, y1, m = y[..., i0].clone(), y[..., i1].clone(), big.clone()
     y[..., i0], y[..., i1] = y0 * c - y1 * sn, y0 * sn + y1 * c
     m[..., i0] = m[..., i1] = big[..., i0] + big[..., i1]
-    return y, (k + 6) * U * m
+    return y, (k + turn) * U * m
 
 
 def rotary_theta(rotary):
@@ -136,7 +139,7 @@ def check_rotate(q, k, rotary, qn, kn, positions=None, first_token=0, **kw):
         if x is None:
             assert y is None
             continue
-        check(y, *ref_rotate64(x, n, rotary, positions, first_token))
+        check(y, *ref_rotate64(x, n, rotary, positions, first_token, y.dtype))
     return got
 
 
@@ -202,7 +205,7 @@ def check_far(q, k, rotary, qn, kn, p):
     for t, (x, n) in enumerate(((q, qn), (k, kn))):
         y, big = ref_norm64(x.double(), n, (1, 3) if n.across_heads else (3,))
         dims = x.shape[1] * x.shape[3] if n.across_heads else x.shape[3]
-        kk = 27 + (96 if n.across_heads else 0) + 2 * math.sqrt(dims) + 6
+        kk = 27 + (96 if n.across_heads else 0) + 2 * math.sqrt(dims) + 7
         for b in range(2):
             for row in rows:
                 ang, ax = [], 0
