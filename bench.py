@@ -77,6 +77,9 @@ def parse():
                         "into the owners' receive buffers and the attention epilogue storing rows into the "
                         "owners' shards (push); the layout pass reading the ranks' projections in place over "
                         "NVLink (p2p); or NCCL all_to_all_single around the call (nccl)")
+    p.add_argument("--conditioned", action="store_true",
+                   help="stack workload: the layers as conditioned blocks, with modulated norm, query/key norm and "
+                        "rotary positions, gate and residual around the attention")
     p.add_argument("--no-e2e", action="store_true")
     p.add_argument("--e2e-copy-streams", type=int, default=3,
                    help="host-to-device copy streams of the e2e leg (the three inputs share them)")
@@ -90,7 +93,10 @@ def parse():
     p.add_argument("--kernel", choices=["select"], default=None,
                    help="time one kernel alone at the workload's shape instead of the layer call (select: "
                         "recap_pool_select on seeded pooled means, about 45 MB on the device)")
-    return p.parse_args()
+    args = p.parse_args()
+    if args.conditioned and not WORKLOADS[args.workload].get("layers"):
+        p.error("--conditioned belongs to the stack workload")
+    return args
 
 
 # ----------------------------------------------------------------------------- data
@@ -702,12 +708,19 @@ class AttentionStack:
     x += heads_to_seq(attend(seq_to_heads(x W_qkv))) W_o, with ``x`` sharded by sequence
     over the ranks and the attention sharded by head (Ulysses).  Random-init projections
     (the benchmark has no checkpoint); the attention is ``recap_b200.Operator.attend``.
-    ``timing`` records CUDA events around each phase of every layer."""
+    ``timing`` records CUDA events around each phase of every layer.
+
+    ``conditioned``: the layers as a model's conditioned blocks have them, with the operators
+    around the attention: a layer norm with scale and shift before the projections, query/key norm and
+    rotary positions over (time, height, width) behind them, and the residual sum through a gate, the next
+    layer's norm on the way: x += gate * attend(...) W_o.  The phases then hold these steps too
+    (the rotation in the exchange towards the heads, the norms in the output projection's)."""
 
     PHASES = ("qkv_projection", "all_to_all_seq_to_heads", "attention", "all_to_all_heads_to_seq",
               "out_projection")
 
-    def __init__(self, op, w: dict, world: int, group, device, exchange: str = "nccl"):
+    def __init__(self, op, w: dict, world: int, group, device, exchange: str = "nccl", conditioned: bool = False):
+        from recap_b200 import AxialRotary, Norm
         from recap_b200.ulysses import PeerBuffer, ShardedIO, check_split
 
         self.op, self.world, self.group = op, world, group
@@ -724,6 +737,19 @@ class AttentionStack:
                       for _ in range(w["layers"])]
         self.w_o = [(torch.randn(hd, self.hidden, generator=g, device=device) * (0.5 / math.sqrt(hd))).to(bf)
                     for _ in range(w["layers"])]
+        self.conditioned = conditioned
+        if conditioned:
+            gb = torch.Generator(device=device).manual_seed(4321)
+            d = self.dim
+            third = 2 * (d // 6)
+            self.rotary = AxialRotary(d, (d - 2 * third, third, third), theta=256.0, grid=w["grid"],
+                                      text_tokens=w["text"], text_first=w["text_first"])
+            self.norm = Norm("layer")
+            self.qk_norms = [tuple(Norm("rms", (1 + 0.1 * torch.randn(d, generator=gb, device=device)).to(bf))
+                                   for _ in range(2)) for _ in range(w["layers"])]
+            # scale, shift, gate of each layer, as the step's conditioning gives them
+            self.mods = [(0.2 * torch.randn(3, self.hidden, generator=gb, device=device)).unbind(0)
+                         for _ in range(w["layers"])]
         self.timing = False
         self.events: list[list] = []
         self.io = None
@@ -764,24 +790,66 @@ class AttentionStack:
             e.record()
             marks.append(e)
 
+    def _norm_in(self, x: torch.Tensor) -> torch.Tensor:
+        """The first layer's input to its projections."""
+        if not self.conditioned:
+            return x
+        from recap_b200 import modulated_norm
+
+        scale, shift, _ = self.mods[0]
+        self.op.launches.count += 1
+        return modulated_norm(x, self.norm, scale=scale, shift=shift)
+
+    def _norm_out(self, layer: int, x: torch.Tensor, y: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """(the layer's residual sum, the next layer's input to its projections) from the projected
+        attention output ``y``."""
+        if not self.conditioned:
+            x = x + y
+            return x, x
+        from recap_b200 import gated_residual
+
+        gate = self.mods[layer][2]
+        self.op.launches.count += 1
+        if layer + 1 == len(self.w_qkv):
+            return gated_residual(x, y, gate)[0], None
+        scale, shift, _ = self.mods[layer + 1]
+        return gated_residual(x, y, gate, norm=self.norm, scale=scale, shift=shift)
+
+    def _turn(self, layer: int, qkv: torch.Tensor, rank: int) -> None:
+        """Query/key norm and rotary positions of this rank's projections, in place."""
+        from recap_b200 import rotate_qk
+
+        q, k = (qkv[:, i].transpose(0, 1).unsqueeze(0) for i in (0, 1))
+        qn, kn = self.qk_norms[layer]
+        self.op.launches.count += 1
+        rotate_qk(q, k, self.rotary, query_norm=qn, key_norm=kn, first_token=rank * self.s, out=(q, k))
+
     def step(self, x: torch.Tensor) -> torch.Tensor:
         """One denoising step's attention layers on this rank's tokens ``[s, hidden]``."""
         from recap_b200.ulysses import heads_to_seq, seq_to_heads
 
         if self.io is not None:
             return self._step_p2p(x)
+        rank = 0
+        if self.group is not None:
+            import torch.distributed as dist
+
+            rank = dist.get_rank(self.group)
+        h = self._norm_in(x)
         for layer in range(len(self.w_qkv)):
             marks: list = []
             self._mark(marks)
-            qkv = (x @ self.w_qkv[layer]).view(self.s, 3, self.heads, self.dim)
+            qkv = (h @ self.w_qkv[layer]).view(self.s, 3, self.heads, self.dim)
             self._mark(marks)
+            if self.conditioned:
+                self._turn(layer, qkv, rank)
             q, k, v = seq_to_heads(qkv, self.world, self.group)
             self._mark(marks)
             o = self.op.attend(layer, q, k, v)
             self._mark(marks)
             y = heads_to_seq(o, self.world, self.group)
             self._mark(marks)
-            x = x + y @ self.w_o[layer]
+            x, h = self._norm_out(layer, x, y @ self.w_o[layer])
             self._mark(marks)
             if self.timing:
                 self.events.append(marks)
@@ -797,21 +865,29 @@ class AttentionStack:
         qkv4 = self.qkv_local if push else io.local_qkv()
         qkv = qkv4.view(self.s, 3 * self.heads * self.dim)
         y = io.local_out()
+        h = self._norm_in(x)
         for layer in range(len(self.w_qkv)):
             marks: list = []
             self._mark(marks)
-            torch.matmul(x, self.w_qkv[layer], out=qkv)
+            torch.matmul(h, self.w_qkv[layer], out=qkv)
             self._mark(marks)
+            turn = {}
+            if self.conditioned:
+                qn, kn = self.qk_norms[layer]
+                turn = dict(rotary=self.rotary, query_norm=qn, key_norm=kn)
+                self.op.launches.count += 1
             if push:
                 # the owners finished reading their receive buffers before the last meeting
-                io.push(qkv4)
+                io.push(qkv4, **turn)
+            elif turn:
+                io.rotate(qkv4, **turn)
             self._meet()  # every shard written (pushed) before any rank reads
             self._mark(marks)
             self.op.attend_sharded(layer, io)
             self._mark(marks)
             self._meet()  # every output row stored, every shard read
             self._mark(marks)
-            x = x + y @ self.w_o[layer]
+            x, h = self._norm_out(layer, x, y @ self.w_o[layer])
             self._mark(marks)
             if self.timing:
                 self.events.append(marks)
@@ -842,7 +918,7 @@ def run_stack(args, w: dict, world: int, rank: int, dev, group) -> None:
                                      text_first=w["text_first"])
     op = Operator.build(OperatorConfig(head_density=w["density"]), SparseGeometry.build(layout, 128),
                         n_layers=w["layers"], process_group=group)
-    stack = AttentionStack(op, w, world, group, dev, exchange=args.exchange)
+    stack = AttentionStack(op, w, world, group, dev, exchange=args.exchange, conditioned=args.conditioned)
     mine = range(rank * stack.s, (rank + 1) * stack.s)
     xs = [stack_hidden(w, mine, w["hidden"], seed=s, device=dev) for s in (0, 1, 2)]
 
@@ -902,7 +978,7 @@ def run_stack(args, w: dict, world: int, rank: int, dev, group) -> None:
             "config": {"workload": w["name"], "layers": w["layers"], "hidden": w["hidden"], "heads": w["heads"],
                        "head_dim": w["dim"], "seq_len": stack.S, "keep": max(1, round(w["density"] * -(-(stack.S - w["text"]) // 128))),
                        "parallelism": f"ulysses sequence/{world} + heads/{world}", "exchange": stack.exchange,
-                       "bank": "HBM",
+                       "bank": "HBM", **({"conditioned": True} if stack.conditioned else {}),
                        "l2": "per-layer inputs > 126 MB L2 (no flush needed)"},
             "us_per_layer": round(sparse_ms * 1000.0 / w["layers"], 1),
             "refresh_step_ms": round(refresh_ms, 2),

@@ -356,7 +356,7 @@ template <typename TI, typename TO, int kLanes, bool kHalves>
 __global__ void __launch_bounds__(kThreads, 4) rotate_across_kernel(const __grid_constant__ RotateArgs a) {
   constexpr int kVec = sizeof(TI) / 2;  // 16-byte slots of a lane's values
   __shared__ uint4 s_pair[kMaxPairs];
-  __shared__ float s_sum[kThreads / kLanes];
+  __shared__ double s_sum[kThreads / kLanes];
   extern __shared__ uint4 s_dynamic[];
   const Place<kLanes, kHalves> me(a);
   const int d0 = me.d0, d1 = me.d1;
@@ -417,22 +417,26 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_across_kernel(const __grid
     }
     widen_pairs<TI, kHalves>(xa, xb, raw);
   };
-  float total = 0.f;
+  // The rows' sums are added in 64 bits, where sums of fp32 values of like size are exact: the result does not
+  // depend on how many groups share a token, so a shard or a chunk of a sequence gives the bits of the whole.
+  double sum = 0.;
 #pragma unroll 2
   for (int i = 0; i < mine; ++i) {
     float xa[4], xb[4];
     read(i, xa, xb);
-    total += square_sum(xa, xb);
+    sum += square_sum(xa, xb);
   }
-  total = lanes_sum<kLanes>(total);
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (!a.token_fast && me.split * kLanes <= 32) {
-    for (int o = kLanes; o < me.split * kLanes; o <<= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    for (int o = kLanes; o < me.split * kLanes; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   } else if (me.split > 1) {
-    if (me.lane == 0) s_sum[me.token * me.split + me.slot] = total;
+    if (me.lane == 0) s_sum[me.token * me.split + me.slot] = sum;
     __syncthreads();
-    total = 0.f;
-    for (int i = 0; i < me.split; ++i) total += s_sum[me.token * me.split + i];
+    sum = 0.;
+    for (int i = 0; i < me.split; ++i) sum += s_sum[me.token * me.split + i];
   }
+  const float total = static_cast<float>(sum);
   const float r = rsqrtf(total / (static_cast<float>(heads) * a.D) + a.eps[t]);
 #pragma unroll
   for (int j = 0; j < 4; ++j) {

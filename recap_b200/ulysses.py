@@ -194,10 +194,27 @@ class ShardedIO:
     def local_out(self) -> torch.Tensor:
         return self.out.local((self.tokens_per_rank, self.total_heads * self.dim), torch.bfloat16)
 
-    def push(self, qkv_local: torch.Tensor) -> None:
+    def rotate(self, qkv_local: torch.Tensor, rotary=None, query_norm=None, key_norm=None) -> None:
+        """Normalise and turn the queries and keys of this rank's projections ``[s, 3, H, d]`` in
+        place (``recap_b200.rotate_qk``), at this rank's place of the sequence: what the model does
+        between its projections and the exchange.  A norm across heads covers all ``H`` heads,
+        which every rank holds for its own tokens."""
+        from .block import rotate_qk
+
+        s, H, d = self.tokens_per_rank, self.total_heads, self.dim
+        if tuple(qkv_local.shape) != (s, 3, H, d):
+            raise ValueError("rotate takes this rank's [s, 3, H, d] projections")
+        if rotary is not None and rotary.sequence_tokens != self.seq:
+            raise ValueError(f"rotary positions of {rotary.sequence_tokens} tokens for a sequence of {self.seq}")
+        q, k = (qkv_local[:, i].transpose(0, 1).unsqueeze(0) for i in (0, 1))
+        rotate_qk(q, k, rotary, query_norm=query_norm, key_norm=key_norm, out=(q, k),
+                  first_token=0 if rotary is None else self.rank * s)
+
+    def push(self, qkv_local: torch.Tensor, *, rotary=None, query_norm=None, key_norm=None) -> None:
         """Push mode: write this rank's ``[s, 3, H, d]`` projections of every head group into
         the receive buffer of the rank that owns it, at this rank's token range: one kernel of
-        16-byte peer stores over NVLink (``recap_push_heads``)."""
+        16-byte peer stores over NVLink (``recap_push_heads``).  With ``rotary`` or the norms
+        the projections are turned in place first (``rotate``)."""
         import ctypes
 
         from . import _lib
@@ -205,6 +222,8 @@ class ShardedIO:
         s, H, d = self.tokens_per_rank, self.total_heads, self.dim
         if tuple(qkv_local.shape) != (s, 3, H, d) or not qkv_local.is_contiguous():
             raise ValueError("push takes this rank's contiguous [s, 3, H, d] projections")
+        if rotary is not None or query_norm is not None or key_norm is not None:
+            self.rotate(qkv_local, rotary, query_norm, key_norm)
         dst = (ctypes.c_void_p * self.world)(*self.recv.ptrs)
         _lib.call("recap_push_heads", _lib.ptr(qkv_local), s, H, d, self.rank, self.world, dst,
                   _lib.stream_handle(qkv_local.device))
