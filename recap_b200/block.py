@@ -23,7 +23,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Sequence
 
 import torch
@@ -39,6 +39,7 @@ _ROTATE_ARGS = struct.Struct("<4Q12qQ3qq4Q10i2f")
 _NORM_ARGS = struct.Struct("<4Q8q3Q6q4Q10i2f")
 
 _TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_POSITIONS = {torch.int32: 32, torch.int64: 64}
 _KINDS = {"rms": 1, "layer": 2}
 _RMS_ACROSS = 3
 
@@ -130,7 +131,7 @@ class AxialRotary:
         self._address = ctypes.addressof(c)
 
 
-@dataclass
+@dataclass(frozen=True, eq=False)
 class Norm:
     """A norm over the last dim: ``"rms"`` (x / sqrt(mean x^2 + eps)) or ``"layer"`` (mean taken off
     first, population variance), times ``weight``, plus ``bias`` (layer norms only).  With
@@ -142,6 +143,7 @@ class Norm:
     bias: torch.Tensor | None = None
     eps: float = 1e-6
     across_heads: bool = False
+    code: int = field(init=False, repr=False, compare=False)  # its RECAP_NORM_* value
 
     def __post_init__(self) -> None:
         if self.kind not in _KINDS:
@@ -152,11 +154,7 @@ class Norm:
             raise ValueError("across_heads is a root mean square norm")
         if not self.eps >= 0.0 or math.isinf(self.eps):
             raise ValueError("eps must be finite and not negative")
-
-    @property
-    def code(self) -> int:
-        """The norm's RECAP_NORM_* value."""
-        return _RMS_ACROSS if self.across_heads else _KINDS[self.kind]
+        object.__setattr__(self, "code", _RMS_ACROSS if self.across_heads else _KINDS[self.kind])
 
 
 def _refuse_gradients(*tensors) -> None:
@@ -182,22 +180,17 @@ def _param(t: torch.Tensor, n: int, device, what: str) -> int:
     return t.data_ptr()
 
 
-def _norm_params(norm: Norm | None, n: int, device) -> tuple[int, int, int]:
-    """(weight address, bias address, their type) of an optional norm."""
-    if norm is None:
-        return 0, 0, 0
+def _norm_params(norm: Norm, n: int, device) -> tuple[int, int, int]:
+    """(weight address, bias address, their type) of a norm."""
     weight, bias = norm.weight, norm.bias
     if weight is None and bias is None:
         return 0, 0, 0
     _refuse_gradients(weight, bias)
-    code = _type((bias if weight is None else weight).dtype, "a norm's weight")
-    if weight is None:
-        return 0, _param(bias, n, device, "norm's bias"), code
-    if bias is None:
-        return _param(weight, n, device, "norm's weight"), 0, code
-    if bias.dtype != weight.dtype:
+    dtype = (bias if weight is None else weight).dtype
+    if weight is not None and bias is not None and bias.dtype != dtype:
         raise ValueError("a norm's weight and bias differ in type")
-    return _param(weight, n, device, "norm's weight"), _param(bias, n, device, "norm's bias"), code
+    return (0 if weight is None else _param(weight, n, device, "norm's weight"),
+            0 if bias is None else _param(bias, n, device, "norm's bias"), _type(dtype, "a norm's weight"))
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
@@ -275,48 +268,57 @@ def rotate_qk(
 
     Returns new tensors in the inputs' token order, of their dtype or of ``out_dtype`` bfloat16; ``out``
     gives them instead: the inputs themselves (in place) or tensors that do not overlap them."""
-    if query.dim() != 4 or query.stride(3) != 1 and query.shape[3] > 1:
+    # (a call on few tokens takes as long as these checks: each tensor property is read once)
+    shape, qs = query.shape, query.stride()
+    if len(shape) != 4 or (qs[3] != 1 and shape[3] > 1):
         raise ValueError("query must be [batch, heads, sequence, dim] with dim contiguous")
-    b, hq, s, d = query.shape
-    hk = 0
+    b, hq, s, d = shape
+    dtype, device = query.dtype, query.device
+    grad = torch.is_grad_enabled()
+    if d % 8 or not 8 <= d <= 256 or hq < 1:
+        raise ValueError("dim must be a multiple of 8 up to 256, and heads positive")
+    hk, ks = 0, (0, 0, 0)
     if key is not None:
-        if key.dim() != 4 or key.stride(3) != 1 and key.shape[3] > 1:
+        shape, ks = key.shape, key.stride()
+        if len(shape) != 4 or (ks[3] != 1 and shape[3] > 1):
             raise ValueError("key must be [batch, heads, sequence, dim] with dim contiguous")
-        hk = key.shape[1]
-        if key.shape[0] != b or key.shape[2] != s or key.shape[3] != d:
+        kb_, hk, s_, d_ = shape
+        if kb_ != b or s_ != s or d_ != d:
             raise ValueError("query and key differ in batch, sequence or dim")
-        if key.dtype != query.dtype or key.device != query.device:
+        if key.dtype != dtype or key.device != device:
             raise ValueError("query and key differ in dtype or device")
         if hk < 1:
             raise ValueError("key has no heads")
-    if d % 8 or not 8 <= d <= 256 or hq < 1:
-        raise ValueError("dim must be a multiple of 8 up to 256, and heads positive")
-    device = query.device
-    in_type = _type(query.dtype, "query")
-    _refuse_gradients(query, key)
+        if grad and key.requires_grad:
+            _refuse_gradients(key)
+    if grad and query.requires_grad:
+        _refuse_gradients(query)
+    in_type = _type(dtype, "query")
     out_type = in_type
-    if out_dtype is not None and out_dtype != query.dtype:
+    if out_dtype is not None and out_dtype != dtype:
         if out_dtype != torch.bfloat16:
             raise ValueError("out_dtype is the inputs' dtype or bfloat16")
         out_type = 0
 
-    if query_norm is None and key_norm is None:
-        code = 0
-    else:
+    code = weight_type = qw = qb = kw = kb = 0
+    q_eps = k_eps = 0.0
+    if query_norm is not None or key_norm is not None:
         if query_norm is None or (key is not None and key_norm is None):
             raise ValueError("query and key are both normalised or neither")
-        code = query_norm.code
-        if key is not None and key_norm.code != code:
-            raise ValueError("the query's and the key's norm differ in kind")
-        if code == _RMS_ACROSS and max(hq, hk) > (256 if d <= 64 else 128 if d <= 128 else 64):
+        code, q_eps = query_norm.code, query_norm.eps
+        across = code == _RMS_ACROSS
+        if across and max(hq, hk) > (256 if d <= 64 else 128 if d <= 128 else 64):
             raise ValueError(f"too many heads of {d} dims for a norm across heads")
-    across = code == _RMS_ACROSS
-    qw, qb, weight_type = _norm_params(query_norm, hq * d if across else d, device)
-    kw, kb, k_type = _norm_params(key_norm if key is not None else None, hk * d if across else d, device)
-    if kw or kb:
-        if (qw or qb) and k_type != weight_type:
-            raise ValueError("the norms' weights differ in type")
-        weight_type = k_type
+        qw, qb, weight_type = _norm_params(query_norm, hq * d if across else d, device)
+        if key is not None:
+            if key_norm.code != code:
+                raise ValueError("the query's and the key's norm differ in kind")
+            k_eps = key_norm.eps
+            kw, kb, k_type = _norm_params(key_norm, hk * d if across else d, device)
+            if kw or kb:
+                if (qw or qb) and k_type != weight_type:
+                    raise ValueError("the norms' weights differ in type")
+                weight_type = k_type
 
     address = bits = at = 0
     pb = ps = pa = 0
@@ -335,11 +337,8 @@ def rotate_qk(
                 raise ValueError("first_token belongs to a grid")
             if positions is None:
                 raise ValueError("a rotary without a grid needs positions")
-            if positions.dtype == torch.int64:
-                bits = 64
-            elif positions.dtype == torch.int32:
-                bits = 32
-            else:
+            bits = _POSITIONS.get(positions.dtype)
+            if bits is None:
                 raise ValueError("positions must be int32 or int64")
             shape, strides = positions.shape, positions.stride()
             if len(shape) == 2:
@@ -368,7 +367,7 @@ def rotate_qk(
                 raise ValueError("out must match query and key, dim contiguous")
             if o.dtype != q_out.dtype or (out_dtype is not None and o.dtype != out_dtype):
                 raise ValueError("out differs in dtype")
-        if q_out.dtype != query.dtype and q_out.dtype != torch.bfloat16:
+        if q_out.dtype != dtype and q_out.dtype != torch.bfloat16:
             raise ValueError("out has the inputs' dtype or bfloat16")
         out_type = _TYPES[q_out.dtype]
         _check_outputs([o for o, _ in pairs], [x for _, x in pairs])
@@ -376,18 +375,15 @@ def rotate_qk(
         raise ValueError("rotate_qk runs on CUDA tensors only")
     if b == 0 or s == 0:
         return q_out, k_out
-    qs, qos = query.stride(), q_out.stride()
-    if key is None:
-        k_ptr = ko_ptr = 0
-        ks = kos = (0, 0, 0)
-    else:
-        k_ptr, ko_ptr, ks, kos = key.data_ptr(), k_out.data_ptr(), key.stride(), k_out.stride()
-    args = _ROTATE_ARGS.pack(
+    qos = q_out.stride()
+    k_ptr = ko_ptr = 0
+    kos = (0, 0, 0)
+    if key is not None:
+        k_ptr, ko_ptr, kos = key.data_ptr(), k_out.data_ptr(), k_out.stride()
+    _run("recap_rotate_qk", device, _ROTATE_ARGS.pack(
         query.data_ptr(), k_ptr, q_out.data_ptr(), ko_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qos[0], qos[1],
         qos[2], kos[0], kos[1], kos[2], at, pb, ps, pa, first_token, qw, qb, kw, kb, b, hq, hk, s, d, in_type, out_type,
-        code, weight_type, bits, query_norm.eps if query_norm is not None else 0.0,
-        key_norm.eps if key_norm is not None else 0.0)
-    _run("recap_rotate_qk", device, args, address)
+        code, weight_type, bits, q_eps, k_eps), address)
     return q_out, k_out
 
 
@@ -403,22 +399,26 @@ def _rows(t: torch.Tensor, shape, device, what: str) -> tuple[int, int]:
     return (0, st[0]) if len(st) == 2 else (st[0], st[1])
 
 
-def _modulation(t: torch.Tensor | None, rows, device, what: str) -> tuple[int, int, int]:
+def _modulation(t: torch.Tensor, rows, device, what: str) -> tuple[int, int, int]:
     """Address and element strides (batch, token; 0 where shared) of a modulation of rows of a shape: one
     vector ``[channels]``, or the rows' dims with size 1 where it is shared."""
-    if t is None:
-        return 0, 0, 0
     shape, st = t.shape, t.stride()
     if t.device != device:
         raise ValueError(f"{what} is on {t.device}, the rows on {device}")
-    if shape[-1:] != rows[-1:] or (st[-1] != 1 and shape[-1] > 1):
+    if not shape or shape[-1] != rows[-1] or (st[-1] != 1 and shape[-1] > 1):
         raise ValueError(f"{what} needs {rows[-1]} contiguous channels")
     if len(shape) == 1:
         return t.data_ptr(), 0, 0
-    if len(shape) != len(rows) or any(m != n and m != 1 for m, n in zip(shape, rows)):
-        raise ValueError(f"{what} has shape {tuple(shape)}, which does not spread over {tuple(rows)}")
-    token = 0 if shape[-2] == 1 else st[-2]
-    return t.data_ptr(), 0 if len(shape) == 2 or shape[0] == 1 else st[0], token
+    if len(shape) == len(rows):
+        token = shape[-2]
+        if token == rows[-2] or token == 1:
+            step = 0 if token == 1 else st[-2]
+            if len(shape) == 2:
+                return t.data_ptr(), 0, step
+            batch = shape[0]
+            if batch == 1 or batch == rows[0]:
+                return t.data_ptr(), 0 if batch == 1 else st[0], step
+    raise ValueError(f"{what} has shape {tuple(shape)}, which does not spread over {tuple(rows)}")
 
 
 def _norm_rows(what: str, x, branch, gate, branch_norm, norm, scale, shift, x_out, h, h_dtype):
@@ -432,29 +432,35 @@ def _norm_rows(what: str, x, branch, gate, branch_norm, norm, scale, shift, x_ou
     x_type, h_type = _type(x.dtype, "rows"), _type(h_dtype, "the norm's output")
     if h_type != x_type and x_type != 2:
         raise ValueError("only float32 rows have a norm or a branch of another type")
-    _refuse_gradients(x, branch, gate, scale, shift)
+    if torch.is_grad_enabled():
+        _refuse_gradients(x, branch, gate, scale, shift)
     xs = _rows(x, shape, device, "rows")
     bs = (0, 0) if branch is None else _rows(branch, shape, device, "branch")
     mod_dtype = None
-    for t in (scale, shift, gate):
-        if t is not None:
-            if mod_dtype is not None and t.dtype != mod_dtype:
-                raise ValueError("scale, shift and gate differ in type")
+    mods = []
+    for t, name in ((scale, "scale"), (shift, "shift"), (gate, "gate")):
+        if t is None:
+            mods.append((0, 0, 0))
+            continue
+        if mod_dtype is None:
             mod_dtype = t.dtype
+        elif t.dtype != mod_dtype:
+            raise ValueError("scale, shift and gate differ in type")
+        mods.append(_modulation(t, shape, device, name))
+    sc, sh, ga = mods
     mod_type = 0 if mod_dtype is None else _type(mod_dtype, "modulations")
-    sc = _modulation(scale, shape, device, "scale")
-    sh = _modulation(shift, shape, device, "shift")
-    ga = _modulation(gate, shape, device, "gate")
-    norm_code = branch_code = 0
+    norm_code = branch_code = w = wb = w_type = bw = bb = b_type = 0
     eps = branch_eps = 0.0
     if norm is not None:
         norm_code, eps = norm.code, norm.eps
+        if norm_code == _RMS_ACROSS:
+            raise ValueError("a norm across heads belongs to rotate_qk")
+        w, wb, w_type = _norm_params(norm, c, device)
     if branch_norm is not None:
         branch_code, branch_eps = branch_norm.code, branch_norm.eps
-    if norm_code == _RMS_ACROSS or branch_code == _RMS_ACROSS:
-        raise ValueError("a norm across heads belongs to rotate_qk")
-    w, wb, w_type = _norm_params(norm, c, device)
-    bw, bb, b_type = _norm_params(branch_norm, c, device)
+        if branch_code == _RMS_ACROSS:
+            raise ValueError("a norm across heads belongs to rotate_qk")
+        bw, bb, b_type = _norm_params(branch_norm, c, device)
     if x_out is not None or h is not None:
         _check_row_outputs(x, branch, (scale, shift, gate), norm, x_out, h, h_dtype)
     b_ptr = xo_ptr = h_ptr = 0
@@ -462,13 +468,19 @@ def _norm_rows(what: str, x, branch, gate, branch_norm, norm, scale, shift, x_ou
     if branch is not None:
         if x_out is None:
             x_out = torch.empty_like(x)
-        xos = _rows(x_out, shape, device, "out")
+            st = x_out.stride()
+            xos = (0, st[0]) if len(st) == 2 else (st[0], st[1])
+        else:
+            xos = _rows(x_out, shape, device, "out")
         b_ptr, xo_ptr = branch.data_ptr(), x_out.data_ptr()
     if norm is not None:
         if h is None:
             like = x if branch is None else branch
             h = torch.empty_like(like) if like.dtype == h_dtype else torch.empty_like(like, dtype=h_dtype)
-        hs = _rows(h, shape, device, "out")
+            st = h.stride()
+            hs = (0, st[0]) if len(st) == 2 else (st[0], st[1])
+        else:
+            hs = _rows(h, shape, device, "out")
         h_ptr = h.data_ptr()
     if not x.is_cuda:
         raise ValueError(f"{what} runs on CUDA tensors only")
