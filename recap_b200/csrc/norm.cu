@@ -10,9 +10,14 @@
 // row lies on one block, kVec times eight values per thread; a block takes kRows tokens of a
 // sample at once, so that their loads are in flight together, their sums share shuffles and
 // barriers, and modulations that tokens share are read once for them.  Modulations of single
-// tokens are loaded with the rows, ahead of the sums.  fp32 rows are read in runs of four values,
-// the next lane's run following: 16 bytes a lane side by side.  h is formed from the fp32 x',
-// not from its rounded copy: one rounding instead of two.
+// tokens are loaded with the rows, ahead of the sums.  Rows of more than eight values a thread wait in
+// shared memory until they are summed (asynchronous copies, each thread of its own values): in
+// registers they left two blocks on an SM (5120 values, fp32 and bf16: 344 us, in shared memory 315 us).
+// fp32 rows are read in runs of four values, the next lane's run following: 16 bytes a lane side by
+// side.  h is formed from the fp32 x', not from its rounded copy: one rounding instead of two.
+// Measured on B200: 32760 tokens of 5120, fp32 residual, bf16 branch and norm: 315 us, 6.4 TB/s, 0.98 of
+// a copy; layer norm of 32760 fp32 rows of 1536 to bf16: 49 us, 6.2 TB/s; both norms, gate and
+// modulations of every token, 17777 rows of 2304 in bf16: 87 us, the rate of a copy.
 #include "elements.cuh"
 
 namespace recap {
@@ -100,6 +105,39 @@ __device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Col
     if (kSplit && live && c.in0) load4(r, row + c.c0);
   }
 }
+// The same by way of the thread's own 16-byte slots of shared memory, `slot` and, for fp32, the one
+// blockDim.x on: copied without waiting, then read.
+constexpr int slots_of(int value_bytes) { return value_bytes / 2; }
+template <bool kSplit, typename T>
+__device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const Columns<kSplit>& c) {
+  if constexpr (sizeof(T) == 4) {
+    if (c.in0) copy16(slot, row + c.c0);
+    if (c.in1) copy16(slot + blockDim.x, row + c.c1);
+  } else if constexpr (kSplit) {
+    if (c.in0) copy8(slot, row + c.c0);
+    if (c.in1) copy8(reinterpret_cast<uint2*>(slot) + 1, row + c.c1);
+  } else {
+    if (c.in0) copy16(slot, row + c.c0);
+  }
+}
+template <bool kSplit, typename T>
+__device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, const Columns<kSplit>& c) {
+  Raw8<T> r;
+  const uint4 a = *slot;
+  r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
+  if constexpr (sizeof(T) == 4) {
+    const uint4 b = slot[blockDim.x];
+    r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
+  }
+  widen8(x, r);
+  if (!c.in1) {  // never copied
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = c.in0 ? x[j] : 0.f;
+      x[j + 4] = 0.f;
+    }
+  }
+}
 template <bool kSplit, typename T>
 __device__ __forceinline__ void store_columns(T* row, const Columns<kSplit>& c, const float (&x)[8]) {
   if (c.in1) {
@@ -175,13 +213,21 @@ __device__ __forceinline__ void add8(float (&x)[8], const float (&p)[8]) {
   for (int j = 0; j < 8; j += 2) add2(x[j], x[j + 1], p[j], p[j + 1]);
 }
 
+// Most threads of a block with eight values each: fp32 rows take up to 80 registers (two blocks of 384 threads),
+// others 64 (two of 512).  The split of a row over threads depends on its length and type only, so a token's sums,
+// and its result, do not depend on how many tokens a call or a block has.
+constexpr int one_vector_threads(int x_bytes) { return x_bytes == 4 ? 384 : 512; }
+
 // How a block comes by its modulations: read when needed, one vector for its tokens (or its one
 // token); or each token's own, of 16 or 32 bits a value, loaded with the rows.
 enum : int { kModsLate = 0, kMods16 = 2, kMods32 = 4 };
 
-template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods>
-__global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm_kernel(const __grid_constant__ NormArgs a) {
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
+__global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr bool kSplit = sizeof(TX) == 4;
+  // wide rows wait in shared memory instead of registers, so that more blocks are resident
+  constexpr bool kStaged = kVec > 1;
+  extern __shared__ uint4 staged[];
   constexpr bool kOwn = kMods != kModsLate;
   __shared__ float buf[2 * kRows * kMaxWarps];
   int turn = 0;
@@ -191,8 +237,10 @@ __global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm
   const int s0 = (blockIdx.x - b * a.blocks) * kRows;
   const int rows = kRows == 1 ? 1 : min(kRows, a.S - s0);
 
-  Raw8<TX> rx[kRows][kVec];
-  Raw8<TH> ry[kGate ? kRows : 1][kVec];
+  Raw8<TX> rx[kStaged ? 1 : kRows][kStaged ? 1 : kVec];
+  Raw8<TH> ry[kStaged || !kGate ? 1 : kRows][kStaged ? 1 : kVec];
+  constexpr int kXSlots = slots_of(sizeof(TX)), kSlots = kXSlots + (kGate ? slots_of(sizeof(TH)) : 0);
+  auto slot = [&](int r, int v) { return staged + (r * kVec + v) * kSlots * blockDim.x + threadIdx.x; };
   {
     const TX* xr = static_cast<const TX*>(a.x) + b * a.x_stride[0] + s0 * a.x_stride[1];
     const TH* yr = nullptr;
@@ -202,13 +250,33 @@ __global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm
 #pragma unroll
       for (int v = 0; v < kVec; ++v) {
         const Columns<kSplit> c(v, C);
-        load_columns<kSplit>(rx[r][v], xr, c, r < rows);
-        if constexpr (kGate) load_columns<kSplit>(ry[r][v], yr, c, r < rows);
+        if constexpr (kStaged) {
+          if (r < rows) {
+            fetch_columns<kSplit>(slot(r, v), xr, c);
+            if constexpr (kGate) fetch_columns<kSplit>(slot(r, v) + kXSlots * blockDim.x, yr, c);
+          }
+        } else {
+          load_columns<kSplit>(rx[r][v], xr, c, r < rows);
+          if constexpr (kGate) load_columns<kSplit>(ry[r][v], yr, c, r < rows);
+        }
       }
       xr += a.x_stride[1];
       if constexpr (kGate) yr += a.branch_stride[1];
     }
   }
+  if constexpr (kStaged) copies_commit();
+  auto row_values = [&](float (&x)[8], int r, int v) {
+    if constexpr (kStaged)
+      read_columns<kSplit, TX>(x, slot(r, v), Columns<kSplit>(v, C));
+    else
+      widen8(x, rx[r][v]);
+  };
+  auto branch_values = [&](float (&x)[8], int r, int v) {
+    if constexpr (kStaged)
+      read_columns<kSplit, TH>(x, slot(r, v) + kXSlots * blockDim.x, Columns<kSplit>(v, C));
+    else
+      widen8(x, ry[r][v]);
+  };
   // modulations of single tokens are as far away as the rows: ask for them now
   uint32_t own[kOwn ? 3 : 1][kOwn ? kRows : 1][kOwn ? kVec : 1][kOwn ? 2 * kMods : 1];
   if constexpr (kOwn) {
@@ -242,11 +310,12 @@ __global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm
 
   float x[kRows][kVec][8];
   float p[8];
+  if constexpr (kStaged) copies_wait<0>();
   if constexpr (kGate) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) widen8(x[r][v], ry[r][v]);
+      for (int v = 0; v < kVec; ++v) branch_values(x[r][v], r, v);
     if (a.branch_norm != kNormNone)
       norm_rows<kRows, kVec, kSplit>(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, turn, warps);
     TX* out = static_cast<TX*>(a.x_out) + b * a.x_out_stride[0] + s0 * a.x_out_stride[1];
@@ -275,7 +344,7 @@ __global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         float res[8];
-        widen8(res, rx[r][v]);
+        row_values(res, r, v);
         add8(x[r][v], res);
         if (r < rows) store_columns<kSplit>(out + r * a.x_out_stride[1], c, x[r][v]);
         if (kSplit && !c.in1) x[r][v][4] = x[r][v][5] = x[r][v][6] = x[r][v][7] = 0.f;  // out of the sums
@@ -286,7 +355,7 @@ __global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
-      for (int v = 0; v < kVec; ++v) widen8(x[r][v], rx[r][v]);
+      for (int v = 0; v < kVec; ++v) row_values(x[r][v], r, v);
   }
   norm_rows<kRows, kVec, kSplit>(x, a.norm == kNormLayer, C, a.eps, buf, turn, warps);
   TH* out = static_cast<TH*>(a.h) + b * a.h_stride[0] + s0 * a.h_stride[1];
@@ -327,33 +396,49 @@ __global__ void __launch_bounds__(kVec == 4 ? 512 : 384, kVec == 4 ? 1 : 2) norm
   }
 }
 
-template <typename TX, typename TH, int kVec, int kRows, int kMods>
-int launch_gate(NormArgs& a, int threads, cudaStream_t s) {
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
+int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
+  auto* kernel = norm_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads>;
   a.blocks = (a.S + kRows - 1) / kRows;
   const unsigned blocks = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.blocks);
-  if (a.branch != nullptr)
-    norm_kernel<TX, TH, kVec, kRows, true, kMods><<<blocks, threads, 0, s>>>(a);
-  else
-    norm_kernel<TX, TH, kVec, kRows, false, kMods><<<blocks, threads, 0, s>>>(a);
+  int smem = 0;
+  if (kVec > 1) {
+    smem = kRows * kVec * (slots_of(sizeof(TX)) + (kGate ? slots_of(sizeof(TH)) : 0)) * threads * 16;
+    if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return kErrLaunch;
+  }
+  kernel<<<blocks, threads, smem, s>>>(a);
   return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+}
+
+template <typename TX, typename TH, int kVec, int kRows, int kMods, int kThreads = kVec == 1 ? one_vector_threads(sizeof(TX)) : 512>
+int launch_gate(NormArgs& a, int threads, cudaStream_t s) {
+  return a.branch != nullptr ? launch_kernel<TX, TH, kVec, kRows, true, kMods, kThreads>(a, threads, s)
+                             : launch_kernel<TX, TH, kVec, kRows, false, kMods, kThreads>(a, threads, s);
 }
 
 template <typename TX, typename TH>
 int launch_vec(NormArgs& a, cudaStream_t s) {
-  // few values a thread, so that a block of up to 384 threads keeps four tokens in registers and two
-  // such blocks fit an SM; longer rows take more values a thread and fewer tokens
-  const int vecs = a.C / 8;
-  const int per = vecs <= 384 ? 1 : vecs <= 768 ? 2 : 4;
-  const int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
   bool shared = true;
   for (int m = 0; m < 3; ++m) shared = shared && (a.mod[m] == nullptr || a.mod_stride[m][1] == 0);
+  // Eight values a thread as far as that goes, sixteen up to 8192 values, else 32: the narrower, the more rows
+  // a block takes and the more blocks are resident.  (B200, bf16 norm with scale and shift, 16384 tokens: 4096
+  // values as 512 threads of eight, four rows a block 51 us, as 256 threads of sixteen, two rows 56 us; bf16
+  // gate and norms of 8192 values as 512 threads of sixteen 215 us, as 256 of 32 287 us.)
+  const int vecs = a.C / 8;
+  const int per = vecs <= one_vector_threads(sizeof(TX)) ? 1 : vecs <= 1024 ? 2 : 4;
+  const int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
   const bool narrow = a.mod_type != kTypeF32;
   // tokens by the block only where blocks of one token would be more than the device holds
   const bool many = static_cast<int64_t>(a.batch) * a.S >= 2048;
   if (per == 1) {
     if (shared) return many ? launch_gate<TX, TH, 1, 4, kModsLate>(a, threads, s) : launch_gate<TX, TH, 1, 1, kModsLate>(a, threads, s);
     if (!narrow) return launch_gate<TX, TH, 1, 1, kMods32>(a, threads, s);
-    return many ? launch_gate<TX, TH, 1, 2, kMods16>(a, threads, s) : launch_gate<TX, TH, 1, 1, kMods16>(a, threads, s);
+    if (!many) return launch_gate<TX, TH, 1, 1, kMods16>(a, threads, s);
+    // two tokens and their modulations in 80 registers rather than 64 as long as blocks are small enough
+    // (2304 values, both norms, bf16: 87 us, in 64 registers 90 us)
+    if (threads <= 384) return launch_gate<TX, TH, 1, 2, kMods16, 384>(a, threads, s);
+    return launch_gate<TX, TH, 1, 2, kMods16>(a, threads, s);
   }
   if (per == 2) {
     if (shared && many) return launch_gate<TX, TH, 2, 2, kModsLate>(a, threads, s);

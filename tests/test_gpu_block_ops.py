@@ -155,12 +155,24 @@ def check_rotate(q, k, rotary, qn, kn, positions=None, first_token=0, **kw):
     ("token", 1, 33, 33, 40, (16, 8, 8)),  # 32 of 40
 ])
 def test_rotate_on_a_grid(dtype, kind, pairs, layout, b, hq, hk, d, dims):
-    if pairs == "halves" and sum(dims) % 8:
-        pytest.fail("the case pairs halves")
     g = _gen(1)
     grid = (3, 4, 5, 2)[:len(dims)]
     text = 7
     rotary = AxialRotary(d, dims, grid=grid, text_tokens=text, text_first=b == 2, pairs=pairs)
+    q, k = make_qk(g, layout, b, hq, hk, rotary.sequence_tokens, d, dtype)
+    check_rotate(q, k, rotary, *make_norms(g, kind, hq, hk, d, dtype))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("kind", ["none", "rms", "layer", "across"])
+@pytest.mark.parametrize("pairs", ["interleaved", "halves"])
+@pytest.mark.parametrize("layout,b,hq,hk,d,dims", [
+    ("packed", 1, 12, 12, 128, (48, 40, 40)), ("head", 2, 33, 7, 40, (8, 16, 16)), ("token", 1, 17, 3, 256, (64, 64, 64)),
+    ("head", 1, 20, 20, 64, (16, 24, 24))])
+def test_rotate_many_tokens(dtype, kind, pairs, layout, b, hq, hk, d, dims):
+    """Enough tokens that a group takes all heads of a token, text and the last tokens inside a block."""
+    g = _gen(19)
+    rotary = AxialRotary(d, dims, grid=(5, 24, 40), text_tokens=9, text_first=b == 2, pairs=pairs)
     q, k = make_qk(g, layout, b, hq, hk, rotary.sequence_tokens, d, dtype)
     check_rotate(q, k, rotary, *make_norms(g, kind, hq, hk, d, dtype))
 
@@ -433,6 +445,33 @@ def test_gated_residual(kind, branch_kind, xt, ht, b, s, c):
         else:
             assert got_h.dtype == ht
             check(got_h, *ref_modulated(want, norm, scale, shift, err))
+
+
+@pytest.mark.parametrize("xt,ht", PAIRS)
+@pytest.mark.parametrize("c", [8, 264, 1352, 3080, 4096, 5120, 8192, 10008])
+def test_many_rows(xt, ht, c):
+    """Enough tokens for blocks of several, with a rest in each sample (701 = 4 * 175 + 1), modulations shared,
+    of a sample, of a token in each type; what each call gives a row does not depend on its neighbours."""
+    g = _gen(18)
+    b, s = 3, 701
+    x, y = rows(g, xt, b, s, c), rows(g, ht, b, s, c)
+    norm, bnorm = row_norm(g, "layer", c, xt), row_norm(g, "rms", c, ht)
+    for shape, mt in [((c,), ht), ((b, 1, c), F32), ((b, s, c), ht), ((b, s, c), F32), ((1, s, c), BF)]:
+        gate, scale, shift = ((0.4 * torch.randn(*shape, generator=g, device=DEV)).to(mt) for _ in range(3))
+        check(modulated_norm(x, norm, scale=scale, shift=shift, out_dtype=ht),
+              *ref_modulated(x.double(), norm, scale, shift, None))
+        got_x, got_h = gated_residual(x, y, gate, branch_norm=bnorm, norm=norm, scale=scale, shift=shift)
+        yy, big = ref_rows(y.double(), bnorm)
+        want = x.double() + gate.double() * yy
+        err = (87 + 2 * math.sqrt(c)) * U * big * gate.double().abs() + 2 * U * ((gate.double() * yy).abs() + want.abs())
+        check(got_x, want, err)
+        check(got_h, *ref_modulated(want, norm, scale, shift, err))
+        # few rows take blocks of one token: the same bits
+        part = [t if t.dim() == 1 else t[1:2, 5:6] if t.shape[1] > 1 and t.shape[0] > 1 else
+                t[:, 5:6] if t.shape[1] > 1 else t[1:2] for t in (gate, scale, shift)]
+        one_x, one_h = gated_residual(x[1:2, 5:6], y[1:2, 5:6], part[0], branch_norm=bnorm, norm=norm, scale=part[1],
+                                      shift=part[2])
+        assert torch.equal(one_x, got_x[1:2, 5:6]) and torch.equal(one_h, got_h[1:2, 5:6])
 
 
 def test_rows_in_place_and_views():
