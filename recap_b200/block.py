@@ -200,20 +200,36 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
 
 
 def _apart(x: torch.Tensor, y: torch.Tensor) -> bool:
-    """Whether two tensors share no element: their spans are apart, or they are the same rows
-    of one packed buffer at different places of each token (``[b, s, 3, h, d]`` projections)."""
+    """Whether two tensors share no element, as far as that can be told: their spans are apart, or
+    they are boxes of one grid (equal strides, each larger than what lies within) that do not meet in
+    some dim, as the parts of a packed projection or of a joint sequence."""
     if x.numel() == 0 or y.numel() == 0:
         return True
     (x0, x1), (y0, y1) = _extent(x), _extent(y)
     if x1 <= y0 or y1 <= x0:
         return True
-    if x.dim() != 4 or x.stride() != y.stride() or x.dtype != y.dtype:
+    if x.dim() != y.dim() or x.dtype != y.dtype or (y0 - x0) % x.element_size():
         return False
-    sb, sh, ss, _ = x.stride()
-    wide = (max(x.shape[1], y.shape[1]) - 1) * sh + x.shape[3]
-    if ss <= 0 or (x.shape[0] > 1 and sb % ss):
-        return False
-    return wide <= (y0 - x0) // x.element_size() % ss <= ss - wide
+    dims = [(s, t, n, m) for s, t, n, m in zip(x.stride(), y.stride(), x.shape, y.shape) if n > 1 or m > 1]
+    dims.sort(reverse=True)
+    away = (y0 - x0) // x.element_size()
+    for i, (step, other, n, m) in enumerate(dims):
+        if step != other or step == 0:
+            return False
+        inner_x = 1 + sum((k - 1) * s for s, _, k, _ in dims[i + 1:])
+        inner_y = 1 + sum((k - 1) * s for s, _, _, k in dims[i + 1:])
+        # y begins `at` steps and `rest` elements from x, with what lies within one step of either in one window
+        # of a step: elements are equal only where their steps are
+        for at in (away // step, away // step + 1):
+            rest = away - at * step
+            if max(inner_x, rest + inner_y) - min(0, rest) <= step:
+                break
+        else:
+            return False
+        if at >= n or -at >= m:
+            return True
+        away = rest
+    return False
 
 
 def _same(x: torch.Tensor, y: torch.Tensor) -> bool:

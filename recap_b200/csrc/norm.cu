@@ -429,8 +429,9 @@ int launch_vec(NormArgs& a, cudaStream_t s) {
   const int per = vecs <= one_vector_threads(sizeof(TX)) ? 1 : vecs <= 1024 ? 2 : 4;
   const int threads = ((vecs + per - 1) / per + 31) / 32 * 32;
   const bool narrow = a.mod_type != kTypeF32;
-  // tokens by the block only where blocks of one token would be more than the device holds
-  const bool many = static_cast<int64_t>(a.batch) * a.S >= 2048;
+  // tokens by the block only where blocks of one token would be more than the device holds, and a sample
+  // fills a block
+  const bool many = static_cast<int64_t>(a.batch) * a.S >= 2048 && a.S >= 4;
   if (per == 1) {
     if (shared) return many ? launch_gate<TX, TH, 1, 4, kModsLate>(a, threads, s) : launch_gate<TX, TH, 1, 1, kModsLate>(a, threads, s);
     if (!narrow) return launch_gate<TX, TH, 1, 1, kMods32>(a, threads, s);

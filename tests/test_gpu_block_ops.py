@@ -331,6 +331,46 @@ def test_rotate_across_many_heads(d, heads):
         check_rotate(q, k, rotary, *make_norms(g, "across", heads, 3, d, dtype))
 
 
+@pytest.mark.parametrize("tokens", [3, 5000])
+def test_rotate_norms_without_weight_or_with_bias_only(tokens):
+    g = _gen(20)
+    rotary = AxialRotary(64, (24, 20, 20), grid=(1, 1, tokens))
+    for dtype in (BF, F32):
+        q, k = make_qk(g, "token", 1, 6, 2, tokens, 64, dtype)
+        bias = torch.randn(64, generator=g, device=DEV)
+        w = 1 + 0.2 * torch.randn(6 * 64, generator=g, device=DEV)
+        check_rotate(q, k, rotary, Norm("rms"), Norm("rms"))
+        check_rotate(q, k, rotary, Norm("layer", None, bias), Norm("layer", None, bias))
+        check_rotate(q, k, rotary, Norm("layer", bias), Norm("layer"))
+        check_rotate(q, k, rotary, Norm("rms", across_heads=True), Norm("rms", across_heads=True))
+        check_rotate(q, k, rotary, Norm("rms", w, across_heads=True), Norm("rms", across_heads=True))
+        check_rotate(q, k, rotary, Norm("rms", across_heads=True, eps=0.3), Norm("rms", w[:128], across_heads=True))
+        check_rotate(q, None, rotary, Norm("rms", w, across_heads=True), None)
+
+
+def test_rotate_constant_and_zero_rows():
+    """A row of equal values has a layer norm of about zero, a row of zeros an rms norm of zero: the epsilon
+    keeps both finite."""
+    q = torch.full((1, 2, 4, 64), 3.0, dtype=BF, device=DEV)
+    got, _ = rotate_qk(q, None, query_norm=Norm("layer"))
+    assert bool((got.abs() <= 0.05).all())  # 3 * 13 u rounded mean over sqrt(eps): 0.0023
+    for n in (Norm("rms"), Norm("rms", across_heads=True)):
+        assert bool((rotate_qk(torch.zeros_like(q), None, query_norm=n)[0] == 0).all())
+
+
+@pytest.mark.parametrize("b,s", [(3000, 1), (700, 3), (420, 5)])
+def test_many_short_samples(b, s):
+    g = _gen(21)
+    x, y = rows(g, F32, b, s, 264), rows(g, BF, b, s, 264)
+    norm = row_norm(g, "layer", 264, F32)
+    gate, scale = (0.4 * torch.randn(b, 1, 264, generator=g, device=DEV) for _ in range(2))
+    got_x, got_h = gated_residual(x, y, gate, norm=norm, scale=scale)
+    want = x.double() + gate.double() * y.double()
+    err = 2 * U * (want.abs() + (want - x.double()).abs())
+    check(got_x, want, err)
+    check(got_h, *ref_modulated(want, norm, scale, None, err))
+
+
 def test_rotate_empty():
     rotary = AxialRotary(64, (16, 24, 24), grid=(2, 5, 7))
     q = torch.empty(0, 3, 70, 64, dtype=BF, device=DEV)
