@@ -26,6 +26,7 @@ import struct
 from dataclasses import dataclass, field
 from typing import Sequence
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -117,16 +118,23 @@ class AxialRotary:
             c.video_tokens = math.prod(self.grid)
             c.video_offset = self.text_tokens if text_first else 0
             self.sequence_tokens = c.video_tokens + self.text_tokens
-        p = 0
-        for axis, d in enumerate(dims):
-            for i in range(d // 2):
-                power = 2.0 * p / sum(dims) if ladder == "shared" else 2.0 * i / d
-                frequency = thetas[axis] ** -power / (2.0 * math.pi)  # turns for each unit of position
-                c.turns[p] = round(math.fmod(frequency * scales[axis], 1.0) * 2.0**64) % 2**64
-                # added to the top 32 bits of the product, which are cut: up makes up for down
-                c.phase[p] = (math.ceil(math.fmod(frequency * starts[axis], 1.0) * 2.0**32) % 2**32) << 32
-                c.axis[p] = axis
-                p += 1
+        n_pairs = sum(dims) // 2
+        axis = np.repeat(np.arange(n), [d // 2 for d in dims])
+        power = 2.0 * np.arange(n_pairs)
+        if ladder == "shared":
+            power /= sum(dims)
+        else:
+            first = np.cumsum((0, *dims[:-1]))  # 2 i of a pair from 2 p
+            power = (power - first[axis]) / np.asarray(dims, dtype=np.float64)[axis]
+        # turns for each unit of position, in 64 bits of a turn (2^64 turns are none)
+        frequency = np.asarray(thetas)[axis] ** -power / (2.0 * math.pi)
+        turns = np.mod(frequency * np.asarray(scales)[axis], 1.0)
+        c.turns[:n_pairs] = [int(x) for x in np.where(turns < 1.0, turns, 0.0) * 2.0**64]
+        if any(starts):
+            # added to the top 32 bits of the product, which are cut: up makes up for down
+            phase = np.ceil(np.mod(frequency * np.asarray(starts)[axis], 1.0) * 2.0**32)
+            c.phase[:n_pairs] = [int(x) % 2**32 << 32 for x in phase]
+        c.axis[:n_pairs] = axis.tolist()
         self._struct = c
         self._address = ctypes.addressof(c)
 
