@@ -26,7 +26,6 @@ import struct
 from dataclasses import dataclass, field
 from typing import Sequence
 
-import numpy as np
 import torch
 
 from . import _lib
@@ -118,23 +117,18 @@ class AxialRotary:
             c.video_tokens = math.prod(self.grid)
             c.video_offset = self.text_tokens if text_first else 0
             self.sequence_tokens = c.video_tokens + self.text_tokens
-        n_pairs = sum(dims) // 2
-        axis = np.repeat(np.arange(n), [d // 2 for d in dims])
-        power = 2.0 * np.arange(n_pairs)
+        total = sum(dims)
         if ladder == "shared":
-            power /= sum(dims)
+            turns = [thetas[0] ** -(2.0 * p / total) / (2.0 * math.pi) for p in range(total // 2)]
         else:
-            first = np.cumsum((0, *dims[:-1]))  # 2 i of a pair from 2 p
-            power = (power - first[axis]) / np.asarray(dims, dtype=np.float64)[axis]
-        # turns for each unit of position, in 64 bits of a turn (2^64 turns are none)
-        frequency = np.asarray(thetas)[axis] ** -power / (2.0 * math.pi)
-        turns = np.mod(frequency * np.asarray(scales)[axis], 1.0)
-        c.turns[:n_pairs] = [int(x) for x in np.where(turns < 1.0, turns, 0.0) * 2.0**64]
+            turns = [theta ** -(2.0 * i / d) / (2.0 * math.pi) for theta, d in zip(thetas, dims) for i in range(d // 2)]
+        axis = [a for a, d in enumerate(dims) for _ in range(d // 2)]
+        # turns for each unit of position, as 64 bits of a turn
+        c.turns[:len(turns)] = [round(f * scales[a] % 1.0 * 2.0**64) % 2**64 for f, a in zip(turns, axis)]
         if any(starts):
             # added to the top 32 bits of the product, which are cut: up makes up for down
-            phase = np.ceil(np.mod(frequency * np.asarray(starts)[axis], 1.0) * 2.0**32)
-            c.phase[:n_pairs] = [int(x) % 2**32 << 32 for x in phase]
-        c.axis[:n_pairs] = axis.tolist()
+            c.phase[:len(turns)] = [math.ceil(f * starts[a] % 1.0 * 2.0**32) % 2**32 << 32 for f, a in zip(turns, axis)]
+        c.axis[:len(turns)] = axis
         self._struct = c
         self._address = ctypes.addressof(c)
 
