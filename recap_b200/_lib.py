@@ -81,6 +81,7 @@ SIGNATURES: dict[str, tuple] = {
 }
 
 _lib = None
+_native = None
 _load_error: Exception | None = None
 
 
@@ -116,10 +117,20 @@ def stream_handle(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def raw_stream(index: int) -> int:
-    """The cudaStream_t of a device's current stream, without a torch Stream object around it (what
-    the launch of a kernel of a few microseconds waits for)."""
-    return torch._C._cuda_getCurrentRawStream(index)
+def native():
+    """The compiled binding of the row kernels around the attention (csrc/binding.cpp), on this library's
+    entry points (once)."""
+    global _native
+    if _native is None:
+        lib = load()
+        try:
+            from . import _native as module
+        except ImportError as error:
+            raise RuntimeError("_native.so is not built; run `python -m recap_b200.build`") from error
+        module.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ("recap_rotate_qk", "recap_norm_rows")),
+                    check)
+        _native = module
+    return _native
 
 
 def check(rc: int, what: str) -> None:

@@ -1,7 +1,8 @@
-"""Build librecap_b200.so in-tree with nvcc for sm_100a.
+"""Build librecap_b200.so in-tree with nvcc for sm_100a, and the compiled binding of its row
+kernels (``_native.so``, C++ over torch) with the host compiler.
 
-Usage: ``python -m recap_b200.build`` (or ``recap_b200.build.build()``).  The library
-is rebuilt when any source under ``recap_b200/csrc`` or ``include/`` is newer than it.
+Usage: ``python -m recap_b200.build`` (or ``recap_b200.build.build()``).  Each is rebuilt
+when a source it comes from, under ``recap_b200/csrc`` or ``include/``, is newer than it.
 """
 
 from __future__ import annotations
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -19,6 +21,8 @@ INCLUDE = REPO_DIR / "include"
 LIB_NAME = "librecap_b200.so"
 LIB_PATH = PACKAGE_DIR / LIB_NAME
 BUILD_DIR = PACKAGE_DIR / "_build"
+BINDING = CSRC / "binding.cpp"
+BINDING_PATH = PACKAGE_DIR / "_native.so"
 
 SOURCES = ["layout.cu", "select.cu", "closure.cu", "cvk.cu", "coarse.cu", "fmha.cu", "refresh.cu", "selftest.cu",
            "exchange.cu", "rotate.cu", "norm.cu", "capi.cu"]
@@ -35,8 +39,12 @@ NVCC_FLAGS = [
 ]
 
 
+def _cuda_home() -> str:
+    return os.environ.get("CUDA_HOME", "/usr/local/cuda")
+
+
 def _nvcc() -> str:
-    cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    cuda_home = _cuda_home()
     cand = Path(cuda_home) / "bin" / "nvcc"
     if cand.exists():
         return str(cand)
@@ -55,8 +63,41 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > built for p in inputs)
 
 
+def _start_binding(force: bool) -> subprocess.Popen | None:
+    """Start compiling the binding if it is out of date."""
+    inputs = [BINDING, INCLUDE / "recap_b200.h", Path(__file__)]
+    if not force and BINDING_PATH.exists() and all(p.stat().st_mtime <= BINDING_PATH.stat().st_mtime for p in inputs):
+        return None
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
+           f"-I{root / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
+           f"-I{Path(_cuda_home()) / 'include'}", str(BINDING), "-o", str(BINDING_PATH.with_suffix(".so.tmp")),
+           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+
+
+def _finish_binding(process: subprocess.Popen | None) -> None:
+    if process is None:
+        return
+    out, _ = process.communicate()
+    if process.returncode != 0:
+        raise RuntimeError("the binding did not compile:\n" + out)
+    os.replace(BINDING_PATH.with_suffix(".so.tmp"), BINDING_PATH)
+
+
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile every kernel source and link the shared library; returns its path."""
+    """Compile the binding and every kernel source and link the shared library; returns its path."""
+    binding = _start_binding(force)
+    try:
+        return _build_library(force, verbose)
+    finally:
+        _finish_binding(binding)
+
+
+def _build_library(force: bool, verbose: bool) -> Path:
     if not force and not _stale():
         return LIB_PATH
     nvcc = _nvcc()

@@ -7,7 +7,7 @@ import struct
 import pytest
 import torch
 
-from recap_b200 import AxialRotary, Norm, _lib, block, gated_residual, modulated_norm, rotate_qk
+from recap_b200 import AxialRotary, Norm, _lib, gated_residual, modulated_norm, rotate_qk
 
 
 def _angle(r: AxialRotary, p: int, position: int) -> float:
@@ -245,7 +245,7 @@ def test_c_abi_rejects_before_any_device_call():
     lib = _lib.load()
     shape, unsupported = _lib.RECAP_ERR_SHAPE, _lib.RECAP_ERR_UNSUPPORTED
     on_grid, on_positions = AxialRotary(64, **GRID), AxialRotary(64, (16, 24))
-    rotary, given = on_grid._address, on_positions._address
+    rotary, given = on_grid._spec[0], on_positions._spec[0]
 
     def rotate(rot=None, **kw):
         return lib.recap_rotate_qk(_rotate_args(**kw), rot, None)
@@ -281,58 +281,29 @@ def test_c_abi_rejects_before_any_device_call():
         assert norm(**kw) == shape, kw
     assert norm(C=16392) == unsupported and norm(ht=2) == unsupported
     assert norm(S=0) == _lib.RECAP_OK and norm(b=0, x=0) == _lib.RECAP_OK
-    assert block._ROTATE_ARGS.size == 248 and block._NORM_ARGS.size == 248
-
-
-def test_calls_make_the_rows_device_current(monkeypatch):
-    """A call on another device than the current one runs with that device current and on its stream."""
-    current, calls = [0], []
-
-    class Device:
-        def __init__(self, device):
-            self.index = torch.device(device).index
-
-        def __enter__(self):
-            self.before, current[0] = current[0], self.index
-
-        def __exit__(self, *exc):
-            current[0] = self.before
-
-    class Lib:
-        @staticmethod
-        def recap_norm_rows(args, stream):
-            calls.append((current[0], stream))
-            return 0
-
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
-    monkeypatch.setattr(torch.cuda, "device", Device)
-    monkeypatch.setattr(_lib, "load", lambda: Lib)
-    monkeypatch.setattr(_lib, "raw_stream", lambda index: 100 + index)
-    block._run("recap_norm_rows", torch.device("cuda", 1), b"")
-    block._run("recap_norm_rows", torch.device("cuda", 0), b"")
-    assert calls == [(1, 101), (0, 100)] and current[0] == 0
 
 
 def test_packed_projections_apart():
     """The overlap test on views of one buffer: packed heads, chunks of tokens, batches."""
+    apart = _lib.native().apart
     qkv = torch.zeros(2, 6, 3, 4, 16)
     q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
-    assert block._apart(q, k) and block._apart(k, q) and block._apart(q, v) and block._apart(v, k)
-    assert not block._apart(q, q) and not block._apart(q, qkv[:, :, 0, 1:].transpose(1, 2))
-    assert block._apart(qkv[0], qkv[1]) and not block._apart(q, qkv)
+    assert apart(q, k) and apart(k, q) and apart(q, v) and apart(v, k)
+    assert not apart(q, q) and not apart(q, qkv[:, :, 0, 1:].transpose(1, 2))
+    assert apart(qkv[0], qkv[1]) and not apart(q, qkv)
     head_major = torch.zeros(2, 4, 6, 16)
-    assert not block._apart(head_major[:, :, :4], head_major[:, :, 2:])
-    assert block._apart(head_major[:, :, :4], head_major[:, :, 4:]) and block._apart(head_major[:, :, 4:], head_major[:, :, :4])
-    assert block._apart(head_major[:, :2], head_major[:, 2:]) and not block._apart(head_major[:, :3], head_major[:, 2:])
+    assert not apart(head_major[:, :, :4], head_major[:, :, 2:])
+    assert apart(head_major[:, :, :4], head_major[:, :, 4:]) and apart(head_major[:, :, 4:], head_major[:, :, :4])
+    assert apart(head_major[:, :2], head_major[:, 2:]) and not apart(head_major[:, :3], head_major[:, 2:])
     joint = torch.zeros(3, 10, 8)
-    assert block._apart(joint[:, :4], joint[:, 4:]) and not block._apart(joint[:, :5], joint[:, 4:])
-    assert block._apart(joint[..., :4], joint[..., 4:]) and not block._apart(joint[..., :5], joint[..., 4:])
-    assert not block._apart(joint[:1].expand(3, 10, 8), joint)
+    assert apart(joint[:, :4], joint[:, 4:]) and not apart(joint[:, :5], joint[:, 4:])
+    assert apart(joint[..., :4], joint[..., 4:]) and not apart(joint[..., :5], joint[..., 4:])
+    assert not apart(joint[:1].expand(3, 10, 8), joint)
     # against the elements themselves, over all pairs of boxes of a small grid
     base = torch.arange(3 * 4 * 5).view(3, 4, 5)
     boxes = [base[a:b, c:d, e:f] for a, b in ((0, 2), (1, 3), (2, 3)) for c, d in ((0, 2), (2, 4), (1, 4))
              for e, f in ((0, 5), (0, 2), (2, 5), (1, 3))]
     for x in boxes:
         for y in boxes:
-            assert block._apart(x, y) == (not set(x.flatten().tolist()) & set(y.flatten().tolist()))
-    assert block._apart(torch.zeros(0, 4, 6, 16), head_major)
+            assert apart(x, y) == (not set(x.flatten().tolist()) & set(y.flatten().tolist()))
+    assert apart(torch.zeros(0, 4, 6, 16), head_major)
