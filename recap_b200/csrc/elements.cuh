@@ -7,6 +7,30 @@
 
 namespace recap {
 
+// Programmatic launch: a kernel launched by launch_after() is set up while the one before it on the stream
+// ends, and every thread waits in grid_wait() until that one is complete and its writes visible, before it
+// touches global memory.  It takes the gap out of calls that follow one another (device times from the stream,
+// us: 69 MB rotation 16.4 -> 14.4, 32760 x 1536 norm 53.2 -> 51.4, 4680 x 1536 gate and norm 20.5 -> 18.1);
+// releasing the next kernel earlier, from inside the running one, gained nothing more.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename Args>
+int launch_after(void (*kernel)(Args), dim3 grid, int threads, int smem, cudaStream_t s, const Args& a) {
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = s;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  if (cudaLaunchKernelEx(&config, kernel, a) == cudaSuccess) return kOk;
+  cudaGetLastError();  // the error goes back as a code, not to a later call
+  return kErrLaunch;
+}
+
 // Two 16-bit values of a 32-bit word <-> fp32 (bf16 widens by a shift; fp16 converts).
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w);

@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   constexpr bool kOwn = kMods != kModsLate;
   __shared__ float buf[2 * kRows * kMaxWarps];
   int turn = 0;
+  grid_wait();
   const int warps = blockDim.x >> 5;
   const int C = a.C;
   const int b = a.batch == 1 ? 0 : blockIdx.x / a.blocks;
@@ -407,8 +408,7 @@ int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
     if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return kErrLaunch;
   }
-  kernel<<<blocks, threads, smem, s>>>(a);
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
+  return launch_after(kernel, dim3(blocks), threads, smem, s, a);
 }
 
 template <typename TX, typename TH, int kVec, int kRows, int kMods, int kThreads = kVec == 1 ? one_vector_threads(sizeof(TX)) : 512>

@@ -248,8 +248,9 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
       if (i0 + i + 1 < mine) src += x_step;
     }
   };
-  load_rows(0);
   stage_pairs(a, s_pair);
+  grid_wait();
+  load_rows(0);
   __syncthreads();
 
   // a pair (u, v) of normalised values before weight and bias becomes
@@ -305,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
         if (i0 + i >= most) break;
         float xa[4], xb[4];
         widen_pairs<TI, kHalves>(xa, xb, raw[i]);
-        float r = 1.f;
+        [[maybe_unused]] float r = 1.f;
         if constexpr (kNorm == kNormLayer) {
           float m0 = 0.f, m1 = 0.f;
 #pragma unroll
@@ -366,6 +367,8 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_across_kernel(const __grid
   const bool weighted = a.weight[t] != nullptr;
   float4* weights = reinterpret_cast<float4*>(s_dynamic) + me.lane;
   uint4* rows = s_dynamic + (weighted ? heads * (2 * kLanes) : 0) + threadIdx.x;
+  stage_pairs(a, s_pair);
+  grid_wait();
   {
     const TI* src = static_cast<const TI*>(a.x[t]) + me.b * a.x_stride[t][0] + me.s * a.x_stride[t][2] + me.slot * a.x_stride[t][1];
     const int64_t x_step = a.x_stride[t][1] << me.log2;
@@ -393,7 +396,6 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_across_kernel(const __grid
       weights[h * (2 * kLanes) + kLanes] = make_float4(wb[0], wb[1], wb[2], wb[3]);
     }
   }
-  stage_pairs(a, s_pair);
   __syncthreads();
 
   float ca[4], sa[4], nsb[4];
@@ -477,11 +479,10 @@ int launch_kernel(const RotateArgs& a, dim3 grid, int smem, cudaStream_t s) {
     auto* kernel = rotate_across_kernel<TI, TO, kLanes, kHalves>;
     if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return kErrLaunch;
-    kernel<<<grid, kThreads, smem, s>>>(a);
+    return launch_after(kernel, grid, kThreads, smem, s, a);
   } else {
-    rotate_kernel<TI, TO, kLanes, kNorm, kHalves><<<grid, kThreads, 0, s>>>(a);
+    return launch_after(rotate_kernel<TI, TO, kLanes, kNorm, kHalves>, grid, kThreads, 0, s, a);
   }
-  return cudaGetLastError() == cudaSuccess ? kOk : kErrLaunch;
 }
 
 template <typename TI, typename TO, int kLanes, int kNorm>

@@ -600,6 +600,45 @@ def test_streams_and_graphs():
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+@pytest.mark.parametrize("s,c", [(3, 512), (700, 512), (9000, 1536)])
+def test_calls_that_follow_one_another(s, c):
+    """A chain of calls, each on what the one before wrote and some in place, torch kernels between them, queued
+    without waiting: the bits of the same chain with a wait after every call."""
+    g = _gen(22)
+    heads = c // 64
+    rotary = AxialRotary(64, (16, 24, 24), grid=(1, 1, s))
+    x0, gate = rows(g, F32, 1, s, c), 0.1 * torch.randn(1, 1, c, generator=g, device=DEV)
+    norm, qn = row_norm(g, "layer", c, F32), Norm("rms", across_heads=True)
+
+    def chain(wait):
+        x = x0.clone()
+        for i in range(12):
+            h = modulated_norm(x, norm, scale=gate, out_dtype=BF)
+            wait()
+            q = h.view(1, s, heads, 64).transpose(1, 2)
+            if i % 3 == 0:
+                h.mul_(0.5)
+                wait()
+            q, _ = rotate_qk(q, None, rotary, query_norm=qn, out=(q, None) if i % 2 else None)
+            wait()
+            x, y = gated_residual(x, q.transpose(1, 2).reshape(1, s, c), gate, norm=norm, out=(x, None))
+            wait()
+            x = x + y.float() if i % 4 == 1 else x
+            wait()
+        return x
+
+    want = chain(torch.cuda.synchronize)
+    for _ in range(5):
+        assert torch.equal(chain(lambda: None), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(lambda: None)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_long_rows_pass_32_bit_offsets():
     """A view whose later rows lie past 2^31 elements of its buffer."""
     g = _gen(15)
