@@ -25,6 +25,7 @@ namespace {
 
 constexpr int kMaxVec = 4;     // vectors of eight values a thread holds of a row
 constexpr int kMaxWarps = 16;  // warps of a row
+constexpr int kTeams = 4;      // warps of a block whose rows take one warp each (15000 rows of 144: 4.6 -> 3.5 us)
 
 // Sums of kRows (1, 2, 4) values over the warp.  Two values share the steps of one: each half of
 // the lanes keeps one value and hands the other over, then goes on with its own.  On return
@@ -73,19 +74,28 @@ __device__ __forceinline__ void block_sum(float (&v)[kRows], float* buf, int war
   for (int r = 0; r < kRows; ++r) v[r] = kRows == 1 ? s : __shfl_sync(0xffffffffu, s, r * kPer);
 }
 
+// The threads of a row: the block's, or, where one warp holds a row, each warp with rows of its own.
+template <bool kWarps>
+struct Team {
+  __device__ __forceinline__ static int threads() { return kWarps ? 32 : blockDim.x; }
+  __device__ __forceinline__ static int me() { return kWarps ? threadIdx.x & 31 : threadIdx.x; }
+  __device__ __forceinline__ static int index() { return kWarps ? threadIdx.x >> 5 : 0; }
+};
+
 // The columns of a thread's vector v: two runs of four values, apart (kSplit) or one after the other.
-template <bool kSplit>
+template <bool kSplit, bool kWarps>
 struct Columns {
   int c0, c1;
   bool in0, in1;
   __device__ __forceinline__ Columns(int v, int C) {
+    const int threads = Team<kWarps>::threads(), me = Team<kWarps>::me();
     if (kSplit) {
-      c0 = (2 * v * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 4;
-      c1 = c0 + 4 * static_cast<int>(blockDim.x);
+      c0 = (2 * v * threads + me) * 4;
+      c1 = c0 + 4 * threads;
       in0 = c0 < C;
       in1 = c1 < C;
     } else {
-      c0 = (v * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
+      c0 = (v * threads + me) * 8;
       c1 = c0 + 4;
       in0 = in1 = c0 < C;
     }
@@ -93,8 +103,8 @@ struct Columns {
 };
 
 // A row's values of those columns, zero past its end.
-template <bool kSplit, typename T>
-__device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Columns<kSplit>& c, bool live) {
+template <bool kSplit, typename T, bool kWarps>
+__device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Columns<kSplit, kWarps>& c, bool live) {
   if (live && c.in1) {
     if constexpr (kSplit)
       load4x2(r, row + c.c0, row + c.c1);
@@ -108,8 +118,8 @@ __device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Col
 // The same by way of the thread's own 16-byte slots of shared memory, `slot` and, for fp32, the one
 // blockDim.x on: copied without waiting, then read.
 constexpr int slots_of(int value_bytes) { return value_bytes / 2; }
-template <bool kSplit, typename T>
-__device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const Columns<kSplit>& c) {
+template <bool kSplit, typename T, bool kWarps>
+__device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const Columns<kSplit, kWarps>& c) {
   if constexpr (sizeof(T) == 4) {
     if (c.in0) copy16(slot, row + c.c0);
     if (c.in1) copy16(slot + blockDim.x, row + c.c1);
@@ -120,8 +130,8 @@ __device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const C
     if (c.in0) copy16(slot, row + c.c0);
   }
 }
-template <bool kSplit, typename T>
-__device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, const Columns<kSplit>& c) {
+template <bool kSplit, typename T, bool kWarps>
+__device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, const Columns<kSplit, kWarps>& c) {
   Raw8<T> r;
   const uint4 a = *slot;
   r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
@@ -138,8 +148,8 @@ __device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, c
     }
   }
 }
-template <bool kSplit, typename T>
-__device__ __forceinline__ void store_columns(T* row, const Columns<kSplit>& c, const float (&x)[8]) {
+template <bool kSplit, typename T, bool kWarps>
+__device__ __forceinline__ void store_columns(T* row, const Columns<kSplit, kWarps>& c, const float (&x)[8]) {
   if (c.in1) {
     if constexpr (kSplit)
       store4x2(row + c.c0, row + c.c1, x);
@@ -151,9 +161,10 @@ __device__ __forceinline__ void store_columns(T* row, const Columns<kSplit>& c, 
 }
 
 // norm(x) in place: the row mean (layer norm), then the mean square, in two sums.
-template <int kRows, int kVec, bool kSplit>
+template <int kRows, int kVec, bool kSplit, bool kWarps>
 __device__ __forceinline__ void norm_rows(float (&x)[kRows][kVec][8], int layer, int C, float eps, float* buf,
-                                          int& turn, int warps) {
+                                          int& turn) {
+  const int warps = Team<kWarps>::threads() >> 5;
   const float inv = 1.f / static_cast<float>(C);
   float t[kRows];
   if (layer) {
@@ -169,7 +180,7 @@ __device__ __forceinline__ void norm_rows(float (&x)[kRows][kVec][8], int layer,
     block_sum(t, buf + (turn ^= kRows * kMaxWarps), warps);
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-      const Columns<kSplit> c(v, C);
+      const Columns<kSplit, kWarps> c(v, C);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const float m = -t[r] * inv;
@@ -213,16 +224,15 @@ __device__ __forceinline__ void add8(float (&x)[8], const float (&p)[8]) {
   for (int j = 0; j < 8; j += 2) add2(x[j], x[j + 1], p[j], p[j + 1]);
 }
 
-// Most threads of a block with eight values each: fp32 rows take up to 80 registers (two blocks of 384 threads),
-// others 64 (two of 512).  The split of a row over threads depends on its length and type only, so a token's sums,
-// and its result, do not depend on how many tokens a call or a block has.
+// Most threads of a block with eight values each.  The split of a row over threads depends on its length and type
+// only, so a token's sums, and its result, do not depend on how many tokens a call or a block has.
 constexpr int one_vector_threads(int x_bytes) { return x_bytes == 4 ? 384 : 512; }
 
 // How a block comes by its modulations: read when needed, one vector for its tokens (or its one
 // token); or each token's own, of 16 or 32 bits a value, loaded with the rows.
 enum : int { kModsLate = 0, kMods16 = 2, kMods32 = 4 };
 
-template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kWarps>
 __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr bool kSplit = sizeof(TX) == 4;
   // wide rows wait in shared memory instead of registers, so that more blocks are resident
@@ -232,11 +242,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   __shared__ float buf[2 * kRows * kMaxWarps];
   int turn = 0;
   grid_wait();
-  const int warps = blockDim.x >> 5;
   const int C = a.C;
   const int b = a.batch == 1 ? 0 : blockIdx.x / a.blocks;
-  const int s0 = (blockIdx.x - b * a.blocks) * kRows;
-  const int rows = kRows == 1 ? 1 : min(kRows, a.S - s0);
+  const int s0 = ((blockIdx.x - b * a.blocks) * (kWarps ? kTeams : 1) + Team<kWarps>::index()) * kRows;
+  const int rows = kRows == 1 && !kWarps ? 1 : min(kRows, a.S - s0);
+  if (kWarps && rows <= 0) return;  // a warp past the last token; it has no barrier to keep
 
   Raw8<TX> rx[kStaged ? 1 : kRows][kStaged ? 1 : kVec];
   Raw8<TH> ry[kStaged || !kGate ? 1 : kRows][kStaged ? 1 : kVec];
@@ -250,7 +260,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
     for (int r = 0; r < kRows; ++r) {
 #pragma unroll
       for (int v = 0; v < kVec; ++v) {
-        const Columns<kSplit> c(v, C);
+        const Columns<kSplit, kWarps> c(v, C);
         if constexpr (kStaged) {
           if (r < rows) {
             fetch_columns<kSplit>(slot(r, v), xr, c);
@@ -268,13 +278,13 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   if constexpr (kStaged) copies_commit();
   auto row_values = [&](float (&x)[8], int r, int v) {
     if constexpr (kStaged)
-      read_columns<kSplit, TX>(x, slot(r, v), Columns<kSplit>(v, C));
+      read_columns<kSplit, TX>(x, slot(r, v), Columns<kSplit, kWarps>(v, C));
     else
       widen8(x, rx[r][v]);
   };
   auto branch_values = [&](float (&x)[8], int r, int v) {
     if constexpr (kStaged)
-      read_columns<kSplit, TH>(x, slot(r, v) + kXSlots * blockDim.x, Columns<kSplit>(v, C));
+      read_columns<kSplit, TH>(x, slot(r, v) + kXSlots * blockDim.x, Columns<kSplit, kWarps>(v, C));
     else
       widen8(x, ry[r][v]);
   };
@@ -289,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
       for (int r = 0; r < kRows; ++r) {
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-          const Columns<kSplit> c(v, C);
+          const Columns<kSplit, kWarps> c(v, C);
           if (r < rows && c.in0) load_own<kSplit, kMods>(own[m][r][v], row, c.c0, c.in1 ? c.c1 : c.c0);
         }
         row += a.mod_stride[m][1] * kMods;
@@ -318,11 +328,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
 #pragma unroll
       for (int v = 0; v < kVec; ++v) branch_values(x[r][v], r, v);
     if (a.branch_norm != kNormNone)
-      norm_rows<kRows, kVec, kSplit>(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, turn, warps);
+      norm_rows<kRows, kVec, kSplit, kWarps>(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, turn);
     TX* out = static_cast<TX*>(a.x_out) + b * a.x_out_stride[0] + s0 * a.x_out_stride[1];
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-      const Columns<kSplit> c(v, C);
+      const Columns<kSplit, kWarps> c(v, C);
       if (!c.in0) continue;
       const int c1 = c.in1 ? c.c1 : c.c0;  // a run past the row reads the one before it and is not stored
       if (a.branch_weight != nullptr) {
@@ -358,11 +368,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
 #pragma unroll
       for (int v = 0; v < kVec; ++v) row_values(x[r][v], r, v);
   }
-  norm_rows<kRows, kVec, kSplit>(x, a.norm == kNormLayer, C, a.eps, buf, turn, warps);
+  norm_rows<kRows, kVec, kSplit, kWarps>(x, a.norm == kNormLayer, C, a.eps, buf, turn);
   TH* out = static_cast<TH*>(a.h) + b * a.h_stride[0] + s0 * a.h_stride[1];
 #pragma unroll
   for (int v = 0; v < kVec; ++v) {
-    const Columns<kSplit> c(v, C);
+    const Columns<kSplit, kWarps> c(v, C);
     if (!c.in0) continue;
     const int c1 = c.in1 ? c.c1 : c.c0;
     if (a.weight != nullptr) {
@@ -397,10 +407,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   }
 }
 
-template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kWarps>
 int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
-  auto* kernel = norm_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads>;
-  a.blocks = (a.S + kRows - 1) / kRows;
+  auto* kernel = norm_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, kWarps>;
+  constexpr int kTokens = kRows * (kWarps ? kTeams : 1);  // of a block
+  a.blocks = (a.S + kTokens - 1) / kTokens;
   const unsigned blocks = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.blocks);
   int smem = 0;
   if (kVec > 1) {
@@ -408,13 +419,24 @@ int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
     if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return kErrLaunch;
   }
-  return launch_after(kernel, dim3(blocks), threads, smem, s, a);
+  return launch_after(kernel, dim3(blocks), kWarps ? 32 * kTeams : threads, smem, s, a);
 }
 
-template <typename TX, typename TH, int kVec, int kRows, int kMods, int kThreads = kVec == 1 ? one_vector_threads(sizeof(TX)) : 512>
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
+int launch_team(NormArgs& a, int threads, cudaStream_t s) {
+  // a row of one warp leaves a block room for others'
+  if constexpr (kVec == 1)
+    if (threads == 32) return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, 32 * kTeams, true>(a, threads, s);
+  return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, false>(a, threads, s);
+}
+
+// Four tokens a block, but two of an fp32 residual and its branch: 64 registers a thread hold no more.  (Gate,
+// layer norm, fp32 residual, 16384 x 2560: 79 us, with four tokens in 80 registers 95 us; gate and norms of bf16,
+// 16384 x 1536: four tokens 36 us, two 38 us.)
+template <typename TX, typename TH, int kVec, int kRows, int kMods, int kThreads = 512>
 int launch_gate(NormArgs& a, int threads, cudaStream_t s) {
-  return a.branch != nullptr ? launch_kernel<TX, TH, kVec, kRows, true, kMods, kThreads>(a, threads, s)
-                             : launch_kernel<TX, TH, kVec, kRows, false, kMods, kThreads>(a, threads, s);
+  if (a.branch == nullptr) return launch_team<TX, TH, kVec, kRows, false, kMods, kThreads>(a, threads, s);
+  return launch_team<TX, TH, kVec, kRows == 4 && sizeof(TX) == 4 ? 2 : kRows, true, kMods, kThreads>(a, threads, s);
 }
 
 template <typename TX, typename TH>

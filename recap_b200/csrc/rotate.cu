@@ -533,18 +533,28 @@ int launch_rotate(RotateArgs& a, cudaStream_t s) {
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   const bool across = a.norm == kNormRmsAcross;
   const int most = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
-  // Share a token's heads among more groups while a group would still have a row of its own and a
-  // tensor's blocks are fewer than the SMs, or while a norm across heads has more rows than it takes.
-  // (Each group forms the token's cosines again: 12 heads of 128, 1560 tokens, rms: 6.2 us; sharing
-  // until two blocks an SM 7.9 us, four 11.3 us; 40 heads, 600 tokens: 7.4 us, not sharing 11.5 us.)
+  // Groups that share a token's heads: the power of two with the least (turns of the device's blocks) *
+  // (instructions of a block: about 80 a row of a group and 330 for a token's cosines, weights and places).  Few tokens
+  // share more; blocks of many rows share where they would need a second turn for a few of them.  (us, not
+  // shared / shared by two / by four / chosen: 40 heads of 128, 600 tokens 11.5 / 8.6 / 7.4 / by four; 5000 tokens
+  // 46.3 / 39.5 / 39.0 / by four; 24 heads, 9400 tokens 39.6 / 39.8 / 46.3 / not; 8 heads, 30000 tokens 44.8 / 52.6 / 81.5 / not.)
+  const int64_t resident = static_cast<int64_t>(sms) * (across || a.in_type == kTypeF32 ? 3 : 4);
+  const int tensors = a.heads[1] > 0 ? 2 : 1;
+  const auto blocks = [&](int l) { return ((tokens << l) + groups - 1) / groups; };
   int log2 = 0;
-  const auto blocks = [&]() { return ((tokens << log2) + groups - 1) / groups; };
-  while ((1 << log2) < groups && (1 << log2) < most &&
-         ((across && (most + (1 << log2) - 1) >> log2 > kAcrossRows) || blocks() < sms))
-    ++log2;
+  int64_t least = -1;
+  for (int l = 0; (1 << l) <= groups && (l == 0 || (1 << (l - 1)) < most); ++l) {
+    const int rows = (most + (1 << l) - 1) >> l;
+    if (across && rows > kAcrossRows && (2 << l) <= groups) continue;
+    const int64_t cost = (blocks(l) * tensors + resident - 1) / resident * (80 * rows + 330);
+    if (least < 0 || cost < least) {
+      least = cost;
+      log2 = l;
+    }
+  }
   a.split_log2 = log2;
   a.token_fast = a.x_stride[0][2] < a.x_stride[0][1];
-  const dim3 grid(static_cast<unsigned>(blocks()), a.heads[1] > 0 ? 2 : 1);
+  const dim3 grid(static_cast<unsigned>(blocks(log2)), tensors);
   int smem = 0;
   if (across) {
     const bool weighted = a.weight[0] != nullptr || a.weight[1] != nullptr;
