@@ -121,9 +121,20 @@ class AxialRotary:
             # added to the top 32 bits of the product, which are cut: up makes up for down
             c.phase[:len(turns)] = [math.ceil(f * starts[a] % 1.0 * 2.0**32) % 2**32 << 32 for f, a in zip(turns, axis)]
         c.axis[:len(turns)] = axis
+        self._arguments = (int(head_dim), dims, thetas, self.grid, self.text_tokens, self.text_first, pairs, ladder, scales,
+                           starts)
         self._struct = c
         # what a call reads of it: the struct's address, and the bounds it checks
         self._spec = (ctypes.addressof(c), self.head_dim, -1 if grid is None else self.sequence_tokens)
+
+    @classmethod
+    def _rebuild(cls, head_dim, dims, theta, grid, text_tokens, text_first, pairs, ladder, scale, start):
+        return cls(head_dim, dims, theta=theta, grid=grid, text_tokens=text_tokens, text_first=text_first, pairs=pairs,
+                   ladder=ladder, scale=scale, start=start)
+
+    def __reduce__(self):
+        # copies and pickles build their own struct: its address is part of the object
+        return AxialRotary._rebuild, self._arguments
 
 
 @dataclass(frozen=True, eq=False)

@@ -54,6 +54,21 @@ def test_grid_of_a_layout():
     assert list(r._struct.grid)[:3] == [3, 4, 5] and r._struct.axes == 3
 
 
+def test_copies_of_a_rotary_stand_alone():
+    """A copied or unpickled rotary has a struct of its own: it outlives the one it came from."""
+    import copy
+    import ctypes
+    import pickle
+
+    r = AxialRotary(96, (32, 24, 24), theta=(1e4, 500.0, 256.0), grid=(2, 3, 4), text_tokens=5, text_first=True,
+                    pairs="halves", scale=(1.0, 0.5, 2.0), start=(0.0, -1.5, 3.0))
+    copies = [copy.copy(r), copy.deepcopy(r), pickle.loads(pickle.dumps(r))]
+    image = bytes(r._struct)
+    for c in copies:
+        assert bytes(c._struct) == image and c._spec[0] == ctypes.addressof(c._struct) != r._spec[0]
+        assert c._spec[1:] == r._spec[1:] and (c.grid, c.axis_dims, c.sequence_tokens) == (r.grid, r.axis_dims, 29)
+
+
 @pytest.mark.parametrize("bad", [
     dict(axis_dims=()), dict(axis_dims=(2,) * 5), dict(axis_dims=(15, 16)), dict(axis_dims=(0, 16)),
     dict(axis_dims=(64, 66)), dict(head_dim=68, axis_dims=(64,)), dict(head_dim=264, axis_dims=(64,)),
