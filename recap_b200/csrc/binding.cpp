@@ -201,6 +201,11 @@ Tensor allocate(const Tensor& like, at::ScalarType dtype) {
   return dtype == like.scalar_type() ? at::empty_like(like) : at::empty_like(like, like.options().dtype(dtype));
 }
 
+// A given tensor is written: autograd's saved copies of it are out of date.
+void written(const Tensor* t) {
+  if (t != nullptr && !t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void raise_code(int rc, const char* name) {
   PyObject* r = PyObject_CallFunction(g_check, "is", rc, name);
   Py_XDECREF(r);
@@ -374,6 +379,8 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       p.D = static_cast<int32_t>(d);
       const int rc = g_rotate(&p, rotary, c10::cuda::getCurrentCUDAStream(device.index()).stream());
       if (rc != RECAP_OK) raise_code(rc, "recap_rotate_qk");
+      written(q_given);
+      if (key != nullptr) written(k_given);
     }
     return pair(&q_out, k_out);
   });
@@ -494,6 +501,8 @@ PyObject* norm_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       p.C = static_cast<int32_t>(c);
       const int rc = g_norm(&p, c10::cuda::getCurrentCUDAStream(device.index()).stream());
       if (rc != RECAP_OK) raise_code(rc, "recap_norm_rows");
+      if (with_branch) written(x_given);
+      written(h_given);
     }
     return pair(x_out, h_out);
   });

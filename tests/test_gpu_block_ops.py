@@ -305,6 +305,26 @@ def test_rotate_in_place_and_into_views(kind):
         assert torch.equal(base[:, :, 2], third)
 
 
+def test_written_outputs_count_as_changed():
+    """Autograd sees that a given tensor was written: a graph that saved it refuses its backward pass."""
+    g = _gen(23)
+    x = torch.randn(1, 4, 64, generator=g, device=DEV)
+    w = torch.randn(64, generator=g, device=DEV, requires_grad=True)
+    for write in (lambda t: modulated_norm(t, Norm("rms"), out=t),
+                  lambda t: gated_residual(t, t.clone(), out=(t, None)),
+                  lambda t: rotate_qk(t.view(1, 1, 4, 64), None, query_norm=Norm("rms"), out=(t.view(1, 1, 4, 64), None))):
+        t = x.clone()
+        loss = (t * w).sum()
+        before = t._version
+        write(t)
+        assert t._version > before
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        t = x.clone()
+        modulated_norm(t, Norm("rms"), out=t)
+
+
 @pytest.mark.parametrize("dtype", [HF, F32])
 def test_rotate_to_bf16(dtype):
     g = _gen(7)
