@@ -123,3 +123,28 @@ def test_conditioned_stack_is_its_operators_in_turn():
         got = stack.step(x0)
         assert torch.equal(got, x) and bool(got.isfinite().all()) and not torch.equal(got, x0)
     op.check_device_status()
+
+
+def test_streamed_banks_with_rotary():
+    """An operator that streams its banks through host memory turns the projections as the resident one."""
+    from recap_b200 import REFRESH, SPARSE, AxialRotary, HostBankOperator, Norm, Operator, OperatorConfig
+    from recap_b200.sparse import Layout, SparseGeometry, hilbert_permutation
+
+    g = torch.Generator(device=DEV).manual_seed(9)
+    grid, d = (4, 16, 16), 64
+    layout = Layout.from_permutation(hilbert_permutation(grid), text_tokens=0, text_first=False)
+    geo = SparseGeometry.build(layout, 128)
+    cfg = OperatorConfig(head_density=0.25)
+    resident, streamed = Operator.build(cfg, geo, n_layers=2), HostBankOperator.build(cfg, geo, n_layers=2)
+    streamed.hbm_budget = 0
+    turn = dict(rotary=AxialRotary(d, (16, 24, 24), grid=grid), query_norm=Norm("rms"), key_norm=Norm("rms"))
+    for step, kind in enumerate((REFRESH, SPARSE, REFRESH)):
+        for op in (resident, streamed):
+            op.begin_step(step, kind)
+        for layer in range(2):
+            q, k, v = (torch.randn(1, 2, 1024, d, generator=g, device=DEV).to(BF) for _ in range(3))
+            with pytest.raises(ValueError):  # refused before anything is written
+                resident.attend(layer, q, k, v, rotary=AxialRotary(d, (16, 24, 24), grid=(4, 16, 15)))
+            assert torch.equal(streamed.attend(layer, q, k, v, **turn), resident.attend(layer, q, k, v, **turn))
+    resident.check_device_status()
+    streamed.check_device_status()
