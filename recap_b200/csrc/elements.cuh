@@ -64,6 +64,22 @@ struct Raw8 {
 __device__ __forceinline__ uint4 ld_v4(const void* p) { return *reinterpret_cast<const uint4*>(p); }
 __device__ __forceinline__ uint2 ld_v2(const void* p) { return *reinterpret_cast<const uint2*>(p); }
 
+// The same for what all blocks read: it stays in L1 while rows stream past (gate and norm of 32760 x 5120, fp32
+// modulations: 304 us, without the hint 306; at the power limit 326 and 330).
+__device__ __forceinline__ uint4 ld_v4_keep(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::evict_last.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint2 ld_v2_keep(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::evict_last.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+
 // Asynchronous copies from global to shared memory, in groups that the issuing thread waits for.
 __device__ __forceinline__ void copy16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -169,14 +185,14 @@ template <bool kSplit>
 __device__ __forceinline__ void load_param_raw(RawParam8& r, const void* p, int64_t at0, int64_t at1, int type) {
   if (type == kTypeF32) {
     const float* f = static_cast<const float*>(p);
-    const uint4 a = ld_v4(f + at0), b = ld_v4(f + (kSplit ? at1 : at0 + 4));
+    const uint4 a = ld_v4_keep(f + at0), b = ld_v4_keep(f + (kSplit ? at1 : at0 + 4));
     r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w, r.w[4] = b.x, r.w[5] = b.y, r.w[6] = b.z, r.w[7] = b.w;
   } else if (kSplit) {
     const uint16_t* h = static_cast<const uint16_t*>(p);
-    const uint2 a = ld_v2(h + at0), b = ld_v2(h + at1);
+    const uint2 a = ld_v2_keep(h + at0), b = ld_v2_keep(h + at1);
     r.w[0] = a.x, r.w[1] = a.y, r.w[2] = b.x, r.w[3] = b.y;
   } else {
-    const uint4 a = ld_v4(static_cast<const uint16_t*>(p) + at0);
+    const uint4 a = ld_v4_keep(static_cast<const uint16_t*>(p) + at0);
     r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
   }
 }

@@ -13,11 +13,15 @@
 // tokens are loaded with the rows, ahead of the sums.  Rows of more than eight values a thread wait in
 // shared memory until they are summed (asynchronous copies, each thread of its own values): in
 // registers they left two blocks on an SM (5120 values, fp32 and bf16: 344 us, in shared memory 315 us).
+// A 16-bit branch beside an fp32 residual waits in registers instead, which leaves room in L1 for the modulations
+// that blocks share (304 us); beside a 16-bit residual it is staged too (16384 x 5120: 122 us, in registers 139 us).
 // fp32 rows are read in runs of four values, the next lane's run following: 16 bytes a lane side by
 // side.  h is formed from the fp32 x', not from its rounded copy: one rounding instead of two.
-// Measured on B200: 32760 tokens of 5120, fp32 residual, bf16 branch and norm: 315 us, 6.4 TB/s, 0.98 of
-// a copy; layer norm of 32760 fp32 rows of 1536 to bf16: 49 us, 6.2 TB/s; both norms, gate and
-// modulations of every token, 17777 rows of 2304 in bf16: 87 us, the rate of a copy.
+// Measured on B200: 32760 tokens of 5120, fp32 residual, bf16 branch and norm: 304 us, 6.6 TB/s; layer norm of
+// 32760 fp32 rows of 1536 to bf16: 46 us, 6.6 TB/s; both norms, gate and modulations of every token, 17777 rows
+// of 2304 in bf16: 87 us, 6.6 TB/s: the rate of a copy.  These are from rest.  After a tenth of a second at this
+// rate the card is at its power limit, the SM clock falls from 1.96 to 1.6 GHz, and the same calls take 326, 47
+// and 92 us (a copy of as many bytes 309, 53 and 94): instructions that are saved are time then.
 #include "elements.cuh"
 
 namespace recap {
@@ -83,7 +87,9 @@ struct Team {
 };
 
 // The columns of a thread's vector v: two runs of four values, apart (kSplit) or one after the other.
-template <bool kSplit, bool kWarps>
+// kWhole: no thread has columns past the row, which takes the selects out of the sums (32760 x 1536, fp32 to bf16:
+// 46 us, with them 47; at the power limit 47 and 49).
+template <bool kSplit, bool kWarps, bool kWhole>
 struct Columns {
   int c0, c1;
   bool in0, in1;
@@ -92,19 +98,19 @@ struct Columns {
     if (kSplit) {
       c0 = (2 * v * threads + me) * 4;
       c1 = c0 + 4 * threads;
-      in0 = c0 < C;
-      in1 = c1 < C;
+      in0 = kWhole || c0 < C;
+      in1 = kWhole || c1 < C;
     } else {
       c0 = (v * threads + me) * 8;
       c1 = c0 + 4;
-      in0 = in1 = c0 < C;
+      in0 = in1 = kWhole || c0 < C;
     }
   }
 };
 
 // A row's values of those columns, zero past its end.
-template <bool kSplit, typename T, bool kWarps>
-__device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Columns<kSplit, kWarps>& c, bool live) {
+template <bool kSplit, typename T, typename C>
+__device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const C& c, bool live) {
   if (live && c.in1) {
     if constexpr (kSplit)
       load4x2(r, row + c.c0, row + c.c1);
@@ -118,8 +124,8 @@ __device__ __forceinline__ void load_columns(Raw8<T>& r, const T* row, const Col
 // The same by way of the thread's own 16-byte slots of shared memory, `slot` and, for fp32, the one
 // blockDim.x on: copied without waiting, then read.
 constexpr int slots_of(int value_bytes) { return value_bytes / 2; }
-template <bool kSplit, typename T, bool kWarps>
-__device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const Columns<kSplit, kWarps>& c) {
+template <bool kSplit, typename T, typename C>
+__device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const C& c) {
   if constexpr (sizeof(T) == 4) {
     if (c.in0) copy16(slot, row + c.c0);
     if (c.in1) copy16(slot + blockDim.x, row + c.c1);
@@ -130,8 +136,8 @@ __device__ __forceinline__ void fetch_columns(uint4* slot, const T* row, const C
     if (c.in0) copy16(slot, row + c.c0);
   }
 }
-template <bool kSplit, typename T, bool kWarps>
-__device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, const Columns<kSplit, kWarps>& c) {
+template <bool kSplit, typename T, typename C>
+__device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, const C& c) {
   Raw8<T> r;
   const uint4 a = *slot;
   r.w[0] = a.x, r.w[1] = a.y, r.w[2] = a.z, r.w[3] = a.w;
@@ -148,8 +154,8 @@ __device__ __forceinline__ void read_columns(float (&x)[8], const uint4* slot, c
     }
   }
 }
-template <bool kSplit, typename T, bool kWarps>
-__device__ __forceinline__ void store_columns(T* row, const Columns<kSplit, kWarps>& c, const float (&x)[8]) {
+template <bool kSplit, typename T, typename C>
+__device__ __forceinline__ void store_columns(T* row, const C& c, const float (&x)[8]) {
   if (c.in1) {
     if constexpr (kSplit)
       store4x2(row + c.c0, row + c.c1, x);
@@ -161,7 +167,7 @@ __device__ __forceinline__ void store_columns(T* row, const Columns<kSplit, kWar
 }
 
 // norm(x) in place: the row mean (layer norm), then the mean square, in two sums.
-template <int kRows, int kVec, bool kSplit, bool kWarps>
+template <int kRows, int kVec, bool kSplit, bool kWarps, bool kWhole>
 __device__ __forceinline__ void norm_rows(float (&x)[kRows][kVec][8], int layer, int C, float eps, float* buf,
                                           int& turn) {
   const int warps = Team<kWarps>::threads() >> 5;
@@ -180,7 +186,7 @@ __device__ __forceinline__ void norm_rows(float (&x)[kRows][kVec][8], int layer,
     block_sum(t, buf + (turn ^= kRows * kMaxWarps), warps);
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-      const Columns<kSplit, kWarps> c(v, C);
+      const Columns<kSplit, kWarps, kWhole> c(v, C);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const float m = -t[r] * inv;
@@ -232,11 +238,17 @@ constexpr int one_vector_threads(int x_bytes) { return x_bytes == 4 ? 384 : 512;
 // token); or each token's own, of 16 or 32 bits a value, loaded with the rows.
 enum : int { kModsLate = 0, kMods16 = 2, kMods32 = 4 };
 
-template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kWarps>
+// Which rows wait in shared memory: wide ones, and four fp32 residuals a block, which registers do not hold.
+template <typename TX, int kVec, int kRows, bool kGate>
+constexpr bool stages() {
+  return kVec > 1 || (kGate && kRows == 4 && sizeof(TX) == 4);
+}
+
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kWarps, bool kWhole>
 __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant__ NormArgs a) {
   constexpr bool kSplit = sizeof(TX) == 4;
-  // wide rows wait in shared memory instead of registers, so that more blocks are resident
-  constexpr bool kStaged = kVec > 1;
+  constexpr bool kStaged = stages<TX, kVec, kRows, kGate>();
+  constexpr bool kStagedBranch = kGate && kStaged && sizeof(TH) == sizeof(TX);
   extern __shared__ uint4 staged[];
   constexpr bool kOwn = kMods != kModsLate;
   __shared__ float buf[2 * kRows * kMaxWarps];
@@ -249,8 +261,8 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   if (kWarps && rows <= 0) return;  // a warp past the last token; it has no barrier to keep
 
   Raw8<TX> rx[kStaged ? 1 : kRows][kStaged ? 1 : kVec];
-  Raw8<TH> ry[kStaged || !kGate ? 1 : kRows][kStaged ? 1 : kVec];
-  constexpr int kXSlots = slots_of(sizeof(TX)), kSlots = kXSlots + (kGate ? slots_of(sizeof(TH)) : 0);
+  Raw8<TH> ry[kStagedBranch || !kGate ? 1 : kRows][kStagedBranch ? 1 : kVec];
+  constexpr int kXSlots = slots_of(sizeof(TX)), kSlots = kXSlots + (kStagedBranch ? slots_of(sizeof(TH)) : 0);
   auto slot = [&](int r, int v) { return staged + (r * kVec + v) * kSlots * blockDim.x + threadIdx.x; };
   {
     const TX* xr = static_cast<const TX*>(a.x) + b * a.x_stride[0] + s0 * a.x_stride[1];
@@ -260,16 +272,16 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
     for (int r = 0; r < kRows; ++r) {
 #pragma unroll
       for (int v = 0; v < kVec; ++v) {
-        const Columns<kSplit, kWarps> c(v, C);
+        const Columns<kSplit, kWarps, kWhole> c(v, C);
         if constexpr (kStaged) {
           if (r < rows) {
             fetch_columns<kSplit>(slot(r, v), xr, c);
-            if constexpr (kGate) fetch_columns<kSplit>(slot(r, v) + kXSlots * blockDim.x, yr, c);
+            if constexpr (kStagedBranch) fetch_columns<kSplit>(slot(r, v) + kXSlots * blockDim.x, yr, c);
           }
         } else {
           load_columns<kSplit>(rx[r][v], xr, c, r < rows);
-          if constexpr (kGate) load_columns<kSplit>(ry[r][v], yr, c, r < rows);
         }
+        if constexpr (kGate && !kStagedBranch) load_columns<kSplit>(ry[r][v], yr, c, r < rows);
       }
       xr += a.x_stride[1];
       if constexpr (kGate) yr += a.branch_stride[1];
@@ -278,13 +290,13 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   if constexpr (kStaged) copies_commit();
   auto row_values = [&](float (&x)[8], int r, int v) {
     if constexpr (kStaged)
-      read_columns<kSplit, TX>(x, slot(r, v), Columns<kSplit, kWarps>(v, C));
+      read_columns<kSplit, TX>(x, slot(r, v), Columns<kSplit, kWarps, kWhole>(v, C));
     else
       widen8(x, rx[r][v]);
   };
   auto branch_values = [&](float (&x)[8], int r, int v) {
-    if constexpr (kStaged)
-      read_columns<kSplit, TH>(x, slot(r, v) + kXSlots * blockDim.x, Columns<kSplit, kWarps>(v, C));
+    if constexpr (kStagedBranch)
+      read_columns<kSplit, TH>(x, slot(r, v) + kXSlots * blockDim.x, Columns<kSplit, kWarps, kWhole>(v, C));
     else
       widen8(x, ry[r][v]);
   };
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
       for (int r = 0; r < kRows; ++r) {
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-          const Columns<kSplit, kWarps> c(v, C);
+          const Columns<kSplit, kWarps, kWhole> c(v, C);
           if (r < rows && c.in0) load_own<kSplit, kMods>(own[m][r][v], row, c.c0, c.in1 ? c.c1 : c.c0);
         }
         row += a.mod_stride[m][1] * kMods;
@@ -321,18 +333,19 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
 
   float x[kRows][kVec][8];
   float p[8];
-  if constexpr (kStaged) copies_wait<0>();
+  if constexpr (kStaged && (!kGate || kStagedBranch)) copies_wait<0>();
   if constexpr (kGate) {
 #pragma unroll
     for (int r = 0; r < kRows; ++r)
 #pragma unroll
       for (int v = 0; v < kVec; ++v) branch_values(x[r][v], r, v);
+    if constexpr (kStaged && !kStagedBranch) copies_wait<0>();
     if (a.branch_norm != kNormNone)
-      norm_rows<kRows, kVec, kSplit, kWarps>(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, turn);
+      norm_rows<kRows, kVec, kSplit, kWarps, kWhole>(x, a.branch_norm == kNormLayer, C, a.branch_eps, buf, turn);
     TX* out = static_cast<TX*>(a.x_out) + b * a.x_out_stride[0] + s0 * a.x_out_stride[1];
 #pragma unroll
     for (int v = 0; v < kVec; ++v) {
-      const Columns<kSplit, kWarps> c(v, C);
+      const Columns<kSplit, kWarps, kWhole> c(v, C);
       if (!c.in0) continue;
       const int c1 = c.in1 ? c.c1 : c.c0;  // a run past the row reads the one before it and is not stored
       if (a.branch_weight != nullptr) {
@@ -368,11 +381,11 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
 #pragma unroll
       for (int v = 0; v < kVec; ++v) row_values(x[r][v], r, v);
   }
-  norm_rows<kRows, kVec, kSplit, kWarps>(x, a.norm == kNormLayer, C, a.eps, buf, turn);
+  norm_rows<kRows, kVec, kSplit, kWarps, kWhole>(x, a.norm == kNormLayer, C, a.eps, buf, turn);
   TH* out = static_cast<TH*>(a.h) + b * a.h_stride[0] + s0 * a.h_stride[1];
 #pragma unroll
   for (int v = 0; v < kVec; ++v) {
-    const Columns<kSplit, kWarps> c(v, C);
+    const Columns<kSplit, kWarps, kWhole> c(v, C);
     if (!c.in0) continue;
     const int c1 = c.in1 ? c.c1 : c.c0;
     if (a.weight != nullptr) {
@@ -407,36 +420,43 @@ __global__ void __launch_bounds__(kThreads, 2) norm_kernel(const __grid_constant
   }
 }
 
-template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kWarps>
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kWarps, bool kWhole>
 int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
-  auto* kernel = norm_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, kWarps>;
+  auto* kernel = norm_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, kWarps, kWhole>;
   constexpr int kTokens = kRows * (kWarps ? kTeams : 1);  // of a block
   a.blocks = (a.S + kTokens - 1) / kTokens;
   const unsigned blocks = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.blocks);
+  const int block = kWarps ? 32 * kTeams : threads;
   int smem = 0;
-  if (kVec > 1) {
-    smem = kRows * kVec * (slots_of(sizeof(TX)) + (kGate ? slots_of(sizeof(TH)) : 0)) * threads * 16;
+  if (stages<TX, kVec, kRows, kGate>()) {
+    smem = kRows * kVec * (slots_of(sizeof(TX)) + (kGate && sizeof(TH) == sizeof(TX) ? slots_of(sizeof(TH)) : 0)) * block * 16;
     if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
       return kErrLaunch;
   }
-  return launch_after(kernel, dim3(blocks), kWarps ? 32 * kTeams : threads, smem, s, a);
+  return launch_after(kernel, dim3(blocks), block, smem, s, a);
 }
 
 template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
 int launch_team(NormArgs& a, int threads, cudaStream_t s) {
   // a row of one warp leaves a block room for others'
   if constexpr (kVec == 1)
-    if (threads == 32) return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, 32 * kTeams, true>(a, threads, s);
-  return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, false>(a, threads, s);
+    if (threads == 32) return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, 32 * kTeams, true, false>(a, threads, s);
+  if (a.C == 8 * kVec * threads) return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, false, true>(a, threads, s);
+  return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, false, false>(a, threads, s);
 }
 
-// Four tokens a block, but two of an fp32 residual and its branch: 64 registers a thread hold no more.  (Gate,
-// layer norm, fp32 residual, 16384 x 2560: 79 us, with four tokens in 80 registers 95 us; gate and norms of bf16,
-// 16384 x 1536: four tokens 36 us, two 38 us.)
+// Four tokens a block, but two of an fp32 residual and its branch, which 64 registers a thread hold; four of them
+// wait in shared memory where an SM takes only two blocks of so many threads, and the branch is of 16 bits.  (Gate,
+// layer norm, fp32 residual, bf16 branch: 16384 x 2560 two tokens 79 us, four staged 80; 16384 x 2568 two tokens 99 us,
+// four staged 89; with an fp32 branch 16384 x 2560 two 100 us, four 101, at the power limit 101 and 105.  Gate and
+// norms of bf16, 16384 x 1536: four tokens 36 us, two 38 us.)
 template <typename TX, typename TH, int kVec, int kRows, int kMods, int kThreads = 512>
 int launch_gate(NormArgs& a, int threads, cudaStream_t s) {
   if (a.branch == nullptr) return launch_team<TX, TH, kVec, kRows, false, kMods, kThreads>(a, threads, s);
-  return launch_team<TX, TH, kVec, kRows == 4 && sizeof(TX) == 4 ? 2 : kRows, true, kMods, kThreads>(a, threads, s);
+  if constexpr (kRows == 4 && sizeof(TX) == 4) {
+    if (sizeof(TH) == 4 || threads <= 320) return launch_team<TX, TH, kVec, 2, true, kMods, kThreads>(a, threads, s);
+  }
+  return launch_team<TX, TH, kVec, kRows, true, kMods, kThreads>(a, threads, s);
 }
 
 template <typename TX, typename TH>
@@ -464,6 +484,10 @@ int launch_vec(NormArgs& a, cudaStream_t s) {
     return launch_gate<TX, TH, 1, 2, kMods16>(a, threads, s);
   }
   if (per == 2) {
+    if constexpr (sizeof(TX) == 2) {
+      // four rows in 96 registers as long as two blocks of that fit (16384 x 5120 bf16: 64 us, two rows 75 us)
+      if (shared && many && a.branch == nullptr && threads <= 320) return launch_team<TX, TH, 2, 4, false, kModsLate, 320>(a, threads, s);
+    }
     if (shared && many) return launch_gate<TX, TH, 2, 2, kModsLate>(a, threads, s);
     if (!shared && narrow) return launch_gate<TX, TH, 2, 1, kMods16>(a, threads, s);
     return launch_gate<TX, TH, 2, 1, kModsLate>(a, threads, s);

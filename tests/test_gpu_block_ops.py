@@ -534,6 +534,13 @@ def test_many_rows(xt, ht, c):
         assert torch.equal(one_x, got_x[1:2, 5:6]) and torch.equal(one_h, got_h[1:2, 5:6])
 
 
+@pytest.mark.parametrize("xt,ht", PAIRS)
+@pytest.mark.parametrize("c", [768, 2568, 2816, 4104, 6144])
+def test_rows_of_whole_blocks(xt, ht, c):
+    """Rows that fill their threads' columns and rows that do not, at the widths where a block takes more tokens."""
+    test_many_rows(xt, ht, c)
+
+
 def test_rows_in_place_and_views():
     g = _gen(12)
     c = 384
