@@ -18,8 +18,9 @@
 // share the heads of one token: more of them where tokens are few.  Next to memory the issue
 // slots count: the arithmetic is packed two values an instruction, and the rows of a warp
 // stay together without branches.  Measured on B200 (bf16): 24 heads of 128, 119056 tokens, rms
-// norm: 441 us, 6.6 TB/s, the rate of a copy; 12 heads, 32760 tokens, rms across heads: 65 us, 6.2
-// TB/s.
+// norm: 441 us, 6.6 TB/s, the rate of a copy; 12 heads, 32760 tokens, rms across heads: 66 us, 6.1
+// TB/s.  Under load for a tenth of a second the card reaches its power limit, the SM clock falls from 1.96
+// to 1.6 GHz, and they take 452 and 71 us.
 #include <type_traits>
 
 #include "elements.cuh"
@@ -220,8 +221,8 @@ __device__ __forceinline__ void turn(float (&xa)[4], float (&xb)[4], const float
 }
 
 // No norm, or one within each head.  One tensor a block (blockIdx.y: q, k).  Four blocks an SM (three
-// for fp32): the layer norm spills six registers for it and is faster all the same (48 heads of 64, two
-// samples of 45106 tokens, fp16: 357 us, 0.95 of the copy rate; three blocks without spills 388 us).
+// for fp32): the layer norm spills some registers for it and is faster all the same (48 heads of 64, two
+// samples of 45106 tokens, fp16: 354 us, 0.96 of the copy rate; three blocks without spills 388 us).
 template <typename TI, typename TO, int kLanes, int kNorm, bool kHalves>
 __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
     rotate_kernel(const __grid_constant__ RotateArgs a) {
@@ -236,21 +237,27 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
   const int mine = me.active ? (heads - me.slot + me.split - 1) >> me.log2 : 0;
   const TI* src = static_cast<const TI*>(a.x[t]) + me.b * a.x_stride[t][0] + me.s * a.x_stride[t][2] +
                   (me.slot < heads ? me.slot : 0) * a.x_stride[t][1];
-  const int64_t x_step = a.x_stride[t][1] << me.log2;
+  // Every group has the same rows, in whole batches: nothing to ask for row by row, in the layer norm of 16-bit rows,
+  // where issue slots count most.  (48 heads of 64, two samples of 45106 tokens, fp16: 354 us, asked 356; at the
+  // card's power limit 377 and 387.  Root mean square: 24 heads of 128 447 and 452, but in halves of 64 42.8 and
+  // 42.1, and fp32 rows 78 and 76 us.)
+  constexpr bool kTryEven = kNorm == kNormLayer && sizeof(TI) == 2;
+  const bool even = kTryEven && heads == (most << me.log2) && most % kBatch == 0;
+  const int64_t x_step = me.active || !even ? a.x_stride[t][1] << me.log2 : 0;
   Raw8<TI> raw[kBatch];
   // A lane without a row of its own loads its last one again: no value has to be made up, and the
   // warp stays together.
-  auto load_rows = [&](int i0) {
+  auto load_rows = [&](int i0, bool whole) {
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (i0 + i >= most) break;
+      if (!whole && i0 + i >= most) break;
       load_row<TI, kHalves>(raw[i], src, d0, d1);
-      if (i0 + i + 1 < mine) src += x_step;
+      if (whole || i0 + i + 1 < mine) src += x_step;
     }
   };
   stage_pairs(a, s_pair);
   grid_wait();
-  load_rows(0);
+  load_rows(0, even);
   __syncthreads();
 
   // a pair (u, v) of normalised values before weight and bias becomes
@@ -298,12 +305,13 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
   const int64_t out_step = a.out_stride[t][1] << me.log2;
   const float inv_d = 1.f / static_cast<float>(a.D);
   const float eps = a.eps[t];
-  auto walk = [&](auto full_tag) {
+  auto walk = [&](auto full_tag, auto even_tag) {
+    constexpr bool kEven = decltype(even_tag)::value;
     for (int i0 = 0; i0 < most; i0 += kBatch) {
-      if (i0 != 0) load_rows(i0);
+      if (i0 != 0) load_rows(i0, kEven);
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        if (i0 + i >= most) break;
+        if (!kEven && i0 + i >= most) break;
         float xa[4], xb[4];
         widen_pairs<TI, kHalves>(xa, xb, raw[i]);
         [[maybe_unused]] float r = 1.f;
@@ -336,15 +344,17 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
             mul2(xb[j], xb[j + 1], r, r);
           }
         }
-        if (i0 + i < mine) store_row<TO, kHalves>(dst, d0, d1, xa, xb);
+        if (kEven ? me.active : i0 + i < mine) store_row<TO, kHalves>(dst, d0, d1, xa, xb);
         dst += out_step;
       }
     }
   };
-  if (full)
-    walk(std::true_type{});
+  if (full && even)
+    walk(std::true_type{}, std::bool_constant<kTryEven>{});
+  else if (full)
+    walk(std::true_type{}, std::false_type{});
   else
-    walk(std::false_type{});
+    walk(std::false_type{}, std::false_type{});
 }
 
 // Root mean square over all heads of a token.  One tensor a block, whose rows go to shared memory by
