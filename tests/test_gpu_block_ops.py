@@ -541,6 +541,47 @@ def test_rows_of_whole_blocks(xt, ht, c):
     test_many_rows(xt, ht, c)
 
 
+@pytest.mark.parametrize("captured", [False, True])
+def test_modulations_written_by_the_call_before(captured):
+    """Calls that follow one another without a gap: what one writes into the modulations, the next reads, also where
+    the one before has read them on every multiprocessor.  The same calls, waited for one by one, give the bits."""
+    g = _gen(31)
+    c, n = 5120, 24
+    x, y = rows(g, F32, 1, 4096, c), rows(g, BF, 1, 4096, c)
+    sources = torch.randn(n, 1, 1, c, generator=g, device=DEV)
+    q = rows(g, BF, 1, 2048, 8 * 64).view(1, 2048, 8, 64).transpose(1, 2)
+    norm, rms = Norm("layer"), Norm("rms")
+    m = torch.zeros(1, 1, c, device=DEV)
+    w = m.view(-1)[:64]
+    head = Norm("rms", w)
+
+    def run(wait):
+        got = []
+        for i in range(n):
+            modulated_norm(sources[i], rms, out=m)
+            wait()
+            _, h = gated_residual(x, y, m, norm=norm, scale=m, shift=m)
+            wait()
+            turned, _ = rotate_qk(q, None, query_norm=head)
+            wait()
+            got += [h[:, ::97, ::13].clone(), turned[:, :, ::61].clone()]
+            wait()
+        return got
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(3):
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = run(lambda: None)
+            graph.replay()
+        else:
+            got = run(lambda: None)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert not torch.equal(want[0], want[2])
+
+
 def test_rows_in_place_and_views():
     g = _gen(12)
     c = 384
