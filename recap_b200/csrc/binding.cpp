@@ -20,6 +20,9 @@
 #include <array>
 #include <cstring>
 #include <string>
+#include <tuple>
+#include <utility>
+#include <vector>
 
 #include "../../include/recap_b200.h"
 
@@ -126,9 +129,11 @@ struct NormParams {
 
 // ------------------------------------------------------------------------------ overlap
 
-// Whether two tensors share no element, as far as that can be told: their spans are apart, or they
-// are boxes of one grid (equal strides, each larger than what lies within) that do not meet in some dim, as
-// the parts of a packed projection or of a joint sequence.
+// Whether two tensors share no element, as far as that can be told.  Dim by dim, the widest steps first: x's elements lie at
+// i step + u and y's at away + j step + v, with u and v what the dims within add, each tensor's by its own strides.  Where
+// the spans of u and of v, moved by what `away` leaves over a step, lie in one window of a step, elements are equal only for i
+// and j that step alike: the tensors are apart if no i and j do, or if those spans do not meet; else the dims within tell.  So
+// the parts of a packed projection or of a joint sequence are told apart, and so are tensors whose dims within differ.
 bool apart(const Tensor& x, const Tensor& y) {
   if (x.numel() == 0 || y.numel() == 0) return true;
   const int64_t size = static_cast<int64_t>(x.element_size());
@@ -142,9 +147,10 @@ bool apart(const Tensor& x, const Tensor& y) {
   const auto [y0, y1] = span(y);
   if (x1 <= y0 || y1 <= x0) return true;
   if (x.dim() != y.dim() || x.scalar_type() != y.scalar_type() || (y0 - x0) % size) return false;
-  std::vector<std::array<int64_t, 4>> dims;  // strides, sizes
+  std::vector<std::array<int64_t, 4>> dims;  // strides, sizes; a dim of one element takes the other's stride
   for (int64_t i = 0; i < x.dim(); ++i)
-    if (x.size(i) > 1 || y.size(i) > 1) dims.push_back({x.stride(i), y.stride(i), x.size(i), y.size(i)});
+    if (x.size(i) > 1 || y.size(i) > 1)
+      dims.push_back({x.size(i) > 1 ? x.stride(i) : y.stride(i), y.size(i) > 1 ? y.stride(i) : x.stride(i), x.size(i), y.size(i)});
   std::sort(dims.rbegin(), dims.rend());
   int64_t away = (y0 - x0) / size;
   for (size_t i = 0; i < dims.size(); ++i) {
@@ -153,10 +159,8 @@ bool apart(const Tensor& x, const Tensor& y) {
     int64_t inner_x = 1, inner_y = 1;
     for (size_t j = i + 1; j < dims.size(); ++j) {
       inner_x += (dims[j][2] - 1) * dims[j][0];
-      inner_y += (dims[j][3] - 1) * dims[j][0];
+      inner_y += (dims[j][3] - 1) * dims[j][1];
     }
-    // y begins `at` steps and `rest` elements from x, with what lies within one step of either in one
-    // window of a step: elements are equal only where their steps are
     int64_t at = away / step - (away % step < 0);
     int64_t rest = 0;
     bool found = false;
@@ -169,6 +173,7 @@ bool apart(const Tensor& x, const Tensor& y) {
     }
     if (!found) return false;
     if (at >= n || -at >= m) return true;
+    if (rest >= inner_x || rest + inner_y <= 0) return true;
     away = rest;
   }
   return false;

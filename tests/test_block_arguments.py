@@ -1,0 +1,59 @@
+"""Arguments of the operators around the attention that have to be refused, or told apart, before any device
+call (no GPU): outputs that overlap, missing operands, foreign types."""
+
+import random
+
+import pytest
+import torch
+
+from recap_b200 import Norm, _lib, modulated_norm
+
+CUDA_ONLY = "CUDA tensors only"  # what a call that is right but for its device meets
+
+
+def _elements(t):
+    at = torch.tensor(t.storage_offset())
+    for n, step in zip(t.shape, t.stride()):
+        at = at.unsqueeze(-1) + torch.arange(n) * step
+    return set(at.flatten().tolist())
+
+
+def test_apart_never_says_so_of_tensors_that_share_an_element():
+    """Pairs of views of one buffer with strides of their own, against the elements themselves."""
+    apart = _lib.native().apart
+    rng = random.Random(5)
+    buf = torch.zeros(4096)
+    told = met = 0
+    for _ in range(30000):
+        n = rng.randint(1, 4)
+        shape = [rng.randint(1, 4) for _ in range(n)]
+        other = shape if rng.random() < 0.7 else [rng.randint(1, 4) for _ in range(n)]
+        steps = rng.sample([1, 2, 3, 4, 6, 8, 12, 16, 24, 48, 64, 96], n)
+        mixed = [s if rng.random() < 0.8 else rng.choice(steps + [0, 1, 8, 32]) for s in steps]
+        x = buf.as_strided(shape, steps, rng.randint(0, 100))
+        y = buf.as_strided(other, mixed, rng.randint(0, 100))
+        meet = bool(_elements(x) & _elements(y))
+        said = apart(x, y)
+        assert not (said and meet), (x.shape, x.stride(), x.storage_offset(), y.shape, y.stride(), y.storage_offset())
+        told += said
+        met += meet
+    assert told > 4000 and met > 4000  # the draw reaches both
+
+
+def test_apart_of_other_orders_within():
+    """The halves of each sample, one in token order and one in head order: apart, though their inner strides differ."""
+    apart = _lib.native().apart
+    w = torch.zeros(3, 2, 6 * 4 * 16)
+    x = w[:, 0].view(3, 6, 4, 16).transpose(1, 2)
+    y = w[:, 1].view(3, 4, 6, 16)
+    assert apart(x, y) and apart(y, x)
+    assert not apart(w[:, 0].view(3, 4, 6, 16), x)
+
+
+def test_output_in_another_order_over_the_input_is_refused():
+    w = torch.zeros(2, 6, 32)
+    x, out = w[:, :, :16], w[1].view(6, 2, 16).transpose(0, 1)
+    with pytest.raises(ValueError, match="overlap"):
+        modulated_norm(x, Norm("rms"), out=out)
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        modulated_norm(x, Norm("rms"), out=w[:, :, 16:])
