@@ -13,7 +13,8 @@ here each is one pass over its rows, in the kernels of ``librecap_b200.so``:
 
 They compute in fp32 and round each output once.  Tensors are bf16, fp16 or fp32 on one
 CUDA device, rows contiguous in their last dim, bases and strides multiples of 16 bytes
-(``ValueError`` otherwise); the kernels run on the current stream of that device.  There is
+(``ValueError`` otherwise); a given output holds each element once, each of its strides larger
+than what the smaller ones span.  The kernels run on the current stream of that device.  There is
 no backward pass, as there is none of ``Operator.attend``: inputs that require a gradient
 while gradients are being recorded raise ``RuntimeError``.
 """

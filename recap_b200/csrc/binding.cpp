@@ -179,11 +179,25 @@ bool apart(const Tensor& x, const Tensor& y) {
   return false;
 }
 
+// Whether a tensor holds each element once: each stride goes past all that the dims of smaller strides span.
+bool distinct(const Tensor& t) {
+  std::vector<std::pair<int64_t, int64_t>> dims;  // strides, sizes
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.size(i) > 1) dims.push_back({t.stride(i), t.size(i)});
+  std::sort(dims.begin(), dims.end());
+  int64_t inner = 1;
+  for (const auto& [step, n] : dims) {
+    if (step < inner) return false;
+    inner += (n - 1) * step;
+  }
+  return true;
+}
+
 bool same(const Tensor& x, const Tensor& y) {
   return x.const_data_ptr() == y.const_data_ptr() && x.strides() == y.strides() && x.scalar_type() == y.scalar_type();
 }
 
-// Outputs hold each element once, may be the input of the same place in the list, and otherwise
+// Outputs hold each element once (distinct()), may be the input of the same place in the list, and otherwise
 // overlap neither an input nor one another.
 template <size_t N>
 void check_outputs(const std::array<const Tensor*, N>& outs, const std::array<const Tensor*, N>& own,
@@ -191,8 +205,7 @@ void check_outputs(const std::array<const Tensor*, N>& outs, const std::array<co
   for (size_t i = 0; i < N; ++i) {
     const Tensor* o = outs[i];
     if (o == nullptr) continue;
-    for (int64_t d = 0; d < o->dim(); ++d)
-      if (o->size(d) > 1 && o->stride(d) == 0) refuse("an output cannot be an expanded tensor");
+    if (o->numel() != 0 && !distinct(*o)) refuse("an output holds an element twice (an expanded tensor, or strides within one another)");
     for (const Tensor* x : inputs)
       if (x != nullptr && !(x == own[i] && same(*o, *x)) && !apart(*o, *x))
         refuse("an output overlaps an input (it may only be that input itself)");

@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from recap_b200 import Norm, _lib, modulated_norm
+from recap_b200 import Norm, _lib, modulated_norm, rotate_qk
 
 CUDA_ONLY = "CUDA tensors only"  # what a call that is right but for its device meets
 
@@ -57,3 +57,20 @@ def test_output_in_another_order_over_the_input_is_refused():
         modulated_norm(x, Norm("rms"), out=out)
     with pytest.raises(ValueError, match=CUDA_ONLY):
         modulated_norm(x, Norm("rms"), out=w[:, :, 16:])
+
+
+@pytest.mark.parametrize("strides", [(96, 8, 1), (8, 16, 1), (80, 16, 1), (0, 16, 1), (96, 0, 1)])
+def test_output_that_holds_an_element_twice_is_refused(strides):
+    out = torch.zeros(1024).as_strided((2, 6, 16), strides)
+    with pytest.raises(ValueError, match="twice"):
+        modulated_norm(torch.zeros(2, 6, 16), Norm("rms"), out=out)
+    q = torch.zeros(1, 2, 6, 16)
+    with pytest.raises(ValueError, match="twice"):
+        rotate_qk(q, None, out=(out.unsqueeze(0), None))
+
+
+@pytest.mark.parametrize("strides", [(96, 16, 1), (16, 32, 1), (1000, 64, 1), (16, 48, 1)])
+def test_output_in_any_order_without_a_second_place_is_taken(strides):
+    out = torch.zeros(4096).as_strided((2, 6, 16), strides)
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        modulated_norm(torch.zeros(2, 6, 16), Norm("rms"), out=out)
