@@ -186,7 +186,8 @@ def rotate_qk(
     takes at most 256, 128 and 64 heads of up to 64, 128 and 256 dims.
 
     Returns new tensors in the inputs' token order, of their dtype or of ``out_dtype`` bfloat16; ``out``
-    gives them instead: the inputs themselves (in place) or tensors that do not overlap them."""
+    gives them instead: the inputs themselves (in place) or tensors that do not overlap them, and in either case
+    neither the norms' parameters nor the positions."""
     q_out, k_out = (None, None) if out is None else out
     if out is not None and q_out is None:
         raise ValueError("out must match query and key, dim contiguous")
@@ -208,7 +209,7 @@ def modulated_norm(
     to 16384.  ``scale`` and ``shift``, of one dtype: ``[channels]``, or the dims of ``x`` with size 1
     where they are shared (``[batch, 1, channels]`` of a sample, ``[batch, tokens, channels]`` of every
     token).  The result has the dtype of ``x``, or for float32 rows ``out_dtype``; ``out`` may be ``x``
-    itself or a tensor that does not overlap the inputs."""
+    itself or a tensor that does not overlap the inputs, the norm's parameters among them."""
     return _lib.native().norm_rows("modulated_norm", x, None, None, None, norm, scale, shift, None, out, out_dtype)[1]
 
 
@@ -229,7 +230,8 @@ def gated_residual(
     ``residual`` and ``branch`` are rows as in ``modulated_norm``; the branch has the residual's dtype, or
     is bf16 or fp16 beside a float32 residual.  ``gate``, ``scale`` and ``shift``, of one dtype, spread
     over the rows as there.  Returns (sum of the residual's dtype, norm of the branch's dtype or None);
-    ``out`` gives either or both: the sum may be the residual itself, the norm the branch itself."""
+    ``out`` gives either or both: the sum may be the residual itself, the norm the branch itself; else they overlap no
+    input, the norms' parameters among them."""
     x_out, h_out = (None, None) if out is None else out
     return _lib.native().norm_rows("gated_residual", residual, branch, gate, branch_norm, norm, scale, shift, x_out, h_out,
                                    None)

@@ -19,8 +19,8 @@
 #include <algorithm>
 #include <array>
 #include <cstring>
+#include <optional>
 #include <string>
-#include <tuple>
 #include <utility>
 #include <vector>
 
@@ -96,11 +96,13 @@ struct Attribute {  // a new reference, released at the end
   Attribute(const Attribute&) = delete;
 };
 
-// A norm's kind, epsilon and parameters of n values each (recap_b200.Norm).
+// A norm's kind, epsilon and parameters of n values each (recap_b200.Norm); holds the parameters.
 struct NormParams {
   int code = RECAP_NORM_NONE, type = 0;
   float eps = 0.f;
   const void *weight = nullptr, *bias = nullptr;
+  const Tensor* tensors[2] = {nullptr, nullptr};  // weight, bias
+  std::optional<Attribute> held[2];
 
   void read(PyObject* norm, int64_t n_head, int64_t n_across, const at::Device& device) {
     {
@@ -110,10 +112,11 @@ struct NormParams {
       if (PyErr_Occurred()) throw Raised{};
     }
     const int64_t n = code == RECAP_NORM_RMS_ACROSS ? n_across : n_head;
-    const Attribute w(norm, s_weight), b(norm, s_bias);
     bool typed = false;
-    for (const auto& [o, to, what] : {std::tuple(w.o, &weight, "norm's weight"), std::tuple(b.o, &bias, "norm's bias")}) {
-      const Tensor* t = tensor(o, what);
+    for (int i = 0; i < 2; ++i) {
+      const char* what = i == 0 ? "norm's weight" : "norm's bias";
+      held[i].emplace(norm, i == 0 ? s_weight : s_bias);
+      const Tensor* t = tensors[i] = tensor(held[i]->o, what);
       if (t == nullptr) continue;
       no_gradient(t);
       if (t->numel() != n || !t->is_contiguous()) refuse(std::string("a ") + what + " must be " + std::to_string(n) + " contiguous values");
@@ -122,7 +125,7 @@ struct NormParams {
       if (typed && code_of != type) refuse("a norm's weight and bias differ in type");
       type = code_of;
       typed = true;
-      *to = t->const_data_ptr();
+      (i == 0 ? weight : bias) = t->const_data_ptr();
     }
   }
 };
@@ -363,7 +366,8 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         if (o->scalar_type() != out_dtype) refuse("out differs in dtype");
         no_gradient(o);
       }
-      check_outputs<2>({q_given, key != nullptr ? k_given : nullptr}, {&query, key}, {&query, key});
+      check_outputs<2>({q_given, key != nullptr ? k_given : nullptr}, {&query, key},
+                       {&query, key, qn.tensors[0], qn.tensors[1], kn.tensors[0], kn.tensors[1], positions});
     } else if (k_given != nullptr) {
       refuse("out must match query and key, dim contiguous");
     }
@@ -490,7 +494,8 @@ PyObject* norm_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         if (h_given->scalar_type() != h_dtype) refuse("the norm's out differs in dtype");
         rows(*h_given, "out", ignored);
       }
-      check_outputs<2>({x_given, h_given}, {&x, with_branch ? branch : &x}, {&x, branch, mods[0], mods[1], mods[2]});
+      check_outputs<2>({x_given, h_given}, {&x, with_branch ? branch : &x}, 
+                       {&x, branch, mods[0], mods[1], mods[2], n.tensors[0], n.tensors[1], bn.tensors[0], bn.tensors[1]});
     }
     if (!x.is_cuda()) refuse(std::string(PyUnicode_AsUTF8(args[0])) + " runs on CUDA tensors only");
     const c10::cuda::CUDAGuard current(device);

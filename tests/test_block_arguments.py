@@ -6,7 +6,7 @@ import random
 import pytest
 import torch
 
-from recap_b200 import Norm, _lib, modulated_norm, rotate_qk
+from recap_b200 import AxialRotary, Norm, _lib, gated_residual, modulated_norm, rotate_qk
 
 CUDA_ONLY = "CUDA tensors only"  # what a call that is right but for its device meets
 
@@ -74,3 +74,30 @@ def test_output_in_any_order_without_a_second_place_is_taken(strides):
     out = torch.zeros(4096).as_strided((2, 6, 16), strides)
     with pytest.raises(ValueError, match=CUDA_ONLY):
         modulated_norm(torch.zeros(2, 6, 16), Norm("rms"), out=out)
+
+
+def test_outputs_over_parameters_or_positions_are_refused():
+    """Blocks read a norm's weight and bias, and the positions, without waiting for one another's rows."""
+    x, w = torch.zeros(2, 3, 16), torch.ones(16)
+    calls = [
+        lambda: modulated_norm(x, Norm("rms", x[0, 0]), out=x),
+        lambda: modulated_norm(x, Norm("layer", w, x[1, 2]), out=x),
+        lambda: modulated_norm(torch.zeros(1, 1, 16), Norm("rms", w), out=w.view(1, 1, 16)),
+        lambda: gated_residual(x, torch.zeros(2, 3, 16), norm=Norm("rms", x[0, 1]), out=(x, None)),
+        lambda: gated_residual(x, torch.zeros(2, 3, 16), branch_norm=Norm("layer", w, x[0, 1]), out=(x, None)),
+    ]
+    q, k = torch.zeros(1, 2, 5, 16), torch.zeros(1, 2, 5, 16)
+    calls += [
+        lambda: rotate_qk(q, k, query_norm=Norm("rms", q[0, 0, 0]), key_norm=Norm("rms"), out=(q, k)),
+        lambda: rotate_qk(q, k, query_norm=Norm("rms", k[0, 0, 0]), key_norm=Norm("rms"), out=(q, k)),
+        lambda: rotate_qk(q, k, query_norm=Norm("layer"), key_norm=Norm("layer", None, q[0, 1, 4]), out=(q, k)),
+    ]
+    flat = torch.zeros(160, dtype=torch.int32)
+    rows = flat.view(torch.float32).view(1, 2, 5, 16)
+    calls.append(lambda: rotate_qk(q, None, AxialRotary(16, (8,)), positions=flat[:5].view(5, 1), out=(rows, None)))
+    for call in calls:
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        rotate_qk(q, k, AxialRotary(16, (8,)), positions=flat[:5].view(5, 1), query_norm=Norm("rms", w),
+                  key_norm=Norm("rms", w), out=(q, k))
