@@ -196,8 +196,11 @@ bool distinct(const Tensor& t) {
   return true;
 }
 
+// Whether two tensors of one shape are the same elements in the same places.
 bool same(const Tensor& x, const Tensor& y) {
-  return x.const_data_ptr() == y.const_data_ptr() && x.strides() == y.strides() && x.scalar_type() == y.scalar_type();
+  for (int64_t i = 0; i < x.dim(); ++i)
+    if (x.size(i) > 1 && x.stride(i) != y.stride(i)) return false;
+  return x.const_data_ptr() == y.const_data_ptr() && x.scalar_type() == y.scalar_type();
 }
 
 // Outputs hold each element once (distinct()), may be the input of the same place in the list, and otherwise

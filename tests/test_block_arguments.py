@@ -101,3 +101,15 @@ def test_outputs_over_parameters_or_positions_are_refused():
     with pytest.raises(ValueError, match=CUDA_ONLY):
         rotate_qk(q, k, AxialRotary(16, (8,)), positions=flat[:5].view(5, 1), query_norm=Norm("rms", w),
                   key_norm=Norm("rms", w), out=(q, k))
+
+
+def test_in_place_through_another_view_of_one_sample():
+    """The stride of a dim of one element says nothing about where the elements lie."""
+    joint = torch.zeros(1, 60, 16)
+    x = joint[:, 10:50]
+    out = x.as_strided(x.shape, (8 * 16, 16, 1), x.storage_offset())
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        modulated_norm(x, Norm("rms"), out=out)
+    q = joint.view(1, 1, 60, 16)
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        rotate_qk(q, None, out=(q.as_strided(q.shape, (16, 16, 16, 1)), None))
