@@ -413,13 +413,14 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 
 // ------------------------------------------------------------------------------ norm_rows
 
-// norm_rows(name, x, branch, gate, branch_norm, norm, scale, shift, x_out, h_out, h_dtype) -> (sum, norm)
+// norm_rows(name, x, branch, gate, branch_norm, norm, scale, shift, x_out, h_out, h_dtype) -> (sum, norm); `branch` False:
+// a norm alone
 PyObject* norm_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     if (n_args != 11) refuse("norm_rows takes 11 arguments");
     const Tensor& x = given(args[1], "rows");
-    const bool with_branch = args[2] != Py_None;
-    const Tensor* branch = tensor(args[2], "branch");
+    const bool with_branch = args[2] != Py_False;
+    const Tensor* branch = with_branch ? &given(args[2], "branch") : nullptr;
     recap_norm_rows_args p;
     std::memset(&p, 0, sizeof(p));
     const int64_t nd = x.dim();

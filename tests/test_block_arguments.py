@@ -113,3 +113,12 @@ def test_in_place_through_another_view_of_one_sample():
     q = joint.view(1, 1, 60, 16)
     with pytest.raises(ValueError, match=CUDA_ONLY):
         rotate_qk(q, None, out=(q.as_strided(q.shape, (16, 16, 16, 1)), None))
+
+
+def test_a_residual_without_a_branch_is_refused():
+    """Not answered by the norm alone, without the residual sum that was asked for."""
+    x = torch.zeros(2, 3, 16)
+    for kw in (dict(norm=Norm("rms")), dict(norm=Norm("rms"), gate=x), dict(branch_norm=Norm("rms"), norm=Norm("rms")),
+               dict(), dict(norm=Norm("rms"), out=(x, None))):
+        with pytest.raises(ValueError, match="branch must be a tensor"):
+            gated_residual(x, None, **kw)
