@@ -15,8 +15,8 @@ They compute in fp32 and round each output once.  Tensors are bf16, fp16 or fp32
 CUDA device, rows contiguous in their last dim, bases and strides multiples of 16 bytes
 (``ValueError`` otherwise); a given output holds each element once, each of its strides larger
 than what the smaller ones span.  The kernels run on the current stream of that device.  There is
-no backward pass, as there is none of ``Operator.attend``: inputs that require a gradient
-while gradients are being recorded raise ``RuntimeError``.
+no backward pass, as there is none of ``Operator.attend``, and no forward-mode derivative: inputs that
+require a gradient while gradients are being recorded, and dual tensors, raise ``RuntimeError``.
 """
 
 from __future__ import annotations

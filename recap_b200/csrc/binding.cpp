@@ -10,6 +10,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -42,6 +43,7 @@ struct Refuse {  // becomes a ValueError
   std::string what;
 };
 struct Recorded {};  // becomes the RuntimeError of an input that requires a gradient
+struct Tangent {};   // becomes the RuntimeError of a dual input
 struct Raised {};    // a Python error is set
 
 [[noreturn]] void refuse(std::string what) { throw Refuse{std::move(what)}; }
@@ -64,8 +66,11 @@ const Tensor& given(PyObject* o, const char* what) {
   return *t;
 }
 
+// Neither a recorded input of a backward pass nor the tangent of a forward one, which is not cut by no_grad().
 void no_gradient(const Tensor* t) {
-  if (t != nullptr && t->requires_grad() && c10::GradMode::is_enabled()) throw Recorded{};
+  if (t == nullptr) return;
+  if (t->requires_grad() && c10::GradMode::is_enabled()) throw Recorded{};
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined()) throw Tangent{};
 }
 
 int type_of(at::ScalarType t, const char* what) {
@@ -264,6 +269,8 @@ PyObject* guarded(F body) {
     PyErr_SetString(PyExc_ValueError, r.what.c_str());
   } catch (const Recorded&) {
     PyErr_SetString(PyExc_RuntimeError, "this operator has no backward pass: call it under torch.no_grad()");
+  } catch (const Tangent&) {
+    PyErr_SetString(PyExc_RuntimeError, "this operator has no forward-mode derivative: give it the primal of a dual tensor");
   } catch (const Raised&) {
   } catch (const std::exception& e) {
     PyErr_SetString(PyExc_RuntimeError, e.what());

@@ -122,3 +122,23 @@ def test_a_residual_without_a_branch_is_refused():
                dict(), dict(norm=Norm("rms"), out=(x, None))):
         with pytest.raises(ValueError, match="branch must be a tensor"):
             gated_residual(x, None, **kw)
+
+
+def test_forward_mode_tangents_are_refused_not_cut():
+    from torch.autograd import forward_ad
+
+    x, q, w = torch.zeros(2, 3, 16), torch.zeros(1, 2, 5, 16), torch.ones(16)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: modulated_norm(dual(x), Norm("rms")), lambda: modulated_norm(x, Norm("rms", dual(w))),
+                     lambda: modulated_norm(x, Norm("rms"), scale=dual(w)), lambda: gated_residual(x, dual(x)),
+                     lambda: gated_residual(x, x, dual(w)), lambda: rotate_qk(dual(q), None),
+                     lambda: rotate_qk(q, dual(q))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(ValueError, match=CUDA_ONLY):
+            modulated_norm(forward_ad.unpack_dual(dual(x)).primal, Norm("rms"))
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        modulated_norm(x, Norm("rms"))
