@@ -92,14 +92,20 @@ int64_t integer(PyObject* o) {
   return v;
 }
 
-struct Attribute {  // a new reference, released at the end
+struct Attribute {  // a new reference, released at the end; `what`: the refusal of an object without it
   PyObject* o;
-  Attribute(PyObject* of, PyObject* name) : o(PyObject_GetAttr(of, name)) {
-    if (o == nullptr) throw Raised{};
+  Attribute(PyObject* of, PyObject* name, const char* what) : o(PyObject_GetAttr(of, name)) {
+    if (o != nullptr) return;
+    if (!PyErr_ExceptionMatches(PyExc_AttributeError)) throw Raised{};
+    PyErr_Clear();
+    refuse(what);
   }
   ~Attribute() { Py_XDECREF(o); }
   Attribute(const Attribute&) = delete;
 };
+
+constexpr const char* kNotANorm = "a norm must be a Norm";
+constexpr const char* kNotARotary = "rotary must be an AxialRotary";
 
 // A norm's kind, epsilon and parameters of n values each (recap_b200.Norm); holds the parameters.
 struct NormParams {
@@ -111,7 +117,7 @@ struct NormParams {
 
   void read(PyObject* norm, int64_t n_head, int64_t n_across, const at::Device& device) {
     {
-      const Attribute c(norm, s_code), e(norm, s_eps);
+      const Attribute c(norm, s_code, kNotANorm), e(norm, s_eps, kNotANorm);
       code = static_cast<int>(integer(c.o));
       eps = static_cast<float>(PyFloat_AsDouble(e.o));
       if (PyErr_Occurred()) throw Raised{};
@@ -120,7 +126,7 @@ struct NormParams {
     bool typed = false;
     for (int i = 0; i < 2; ++i) {
       const char* what = i == 0 ? "norm's weight" : "norm's bias";
-      held[i].emplace(norm, i == 0 ? s_weight : s_bias);
+      held[i].emplace(norm, i == 0 ? s_weight : s_bias, kNotANorm);
       const Tensor* t = tensors[i] = tensor(held[i]->o, what);
       if (t == nullptr) continue;
       no_gradient(t);
@@ -336,8 +342,8 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const Tensor* positions = tensor(args[5], "positions");
     p.first_token = integer(args[6]);
     if (args[2] != Py_None) {
-      const Attribute spec(args[2], s_spec);  // (address, head dim, sequence tokens of the grid or -1)
-      if (!PyTuple_Check(spec.o) || PyTuple_GET_SIZE(spec.o) != 3) refuse("rotary must be an AxialRotary");
+      const Attribute spec(args[2], s_spec, kNotARotary);  // (address, head dim, sequence tokens of the grid or -1)
+      if (!PyTuple_Check(spec.o) || PyTuple_GET_SIZE(spec.o) != 3) refuse(kNotARotary);
       rotary = reinterpret_cast<const recap_rotary*>(integer(PyTuple_GET_ITEM(spec.o, 0)));
       const int64_t head_dim = integer(PyTuple_GET_ITEM(spec.o, 1)), tokens = integer(PyTuple_GET_ITEM(spec.o, 2));
       if (head_dim != d) refuse("rotary positions of " + std::to_string(head_dim) + " dims on heads of " + std::to_string(d));

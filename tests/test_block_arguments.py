@@ -142,3 +142,15 @@ def test_forward_mode_tangents_are_refused_not_cut():
             modulated_norm(forward_ad.unpack_dual(dual(x)).primal, Norm("rms"))
     with pytest.raises(ValueError, match=CUDA_ONLY):
         modulated_norm(x, Norm("rms"))
+
+
+def test_foreign_objects_are_refused():
+    x, q = torch.zeros(2, 3, 16), torch.zeros(1, 2, 5, 16)
+    for other in (object(), "rms", torch.nn.LayerNorm(16), torch.zeros(16)):
+        for call in (lambda: modulated_norm(x, other), lambda: gated_residual(x, x, norm=other),
+                     lambda: gated_residual(x, x, branch_norm=other),
+                     lambda: rotate_qk(q, None, query_norm=other)):
+            with pytest.raises(ValueError, match="must be a Norm"):
+                call()
+        with pytest.raises(ValueError, match="must be an AxialRotary"):
+            rotate_qk(q, None, other)
