@@ -210,7 +210,7 @@ def modulated_norm(
     where they are shared (``[batch, 1, channels]`` of a sample, ``[batch, tokens, channels]`` of every
     token).  The result has the dtype of ``x``, or for float32 rows ``out_dtype``; ``out`` may be ``x``
     itself or a tensor that does not overlap the inputs, the norm's parameters among them."""
-    return _lib.native().norm_rows("modulated_norm", x, False, None, None, norm, scale, shift, None, out, out_dtype)[1]
+    return _lib.native().norm_rows("modulated_norm", x, None, None, None, norm, scale, shift, None, out, out_dtype)[1]
 
 
 def gated_residual(

@@ -426,13 +426,13 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 
 // ------------------------------------------------------------------------------ norm_rows
 
-// norm_rows(name, x, branch, gate, branch_norm, norm, scale, shift, x_out, h_out, h_dtype) -> (sum, norm); `branch` False:
-// a norm alone
+// norm_rows(name, x, branch, gate, branch_norm, norm, scale, shift, x_out, h_out, h_dtype) -> (sum, norm); the name is
+// "gated_residual", with a branch, or "modulated_norm", without
 PyObject* norm_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     if (n_args != 11) refuse("norm_rows takes 11 arguments");
     const Tensor& x = given(args[1], "rows");
-    const bool with_branch = args[2] != Py_False;
+    const bool with_branch = PyUnicode_CompareWithASCIIString(args[0], "gated_residual") == 0;
     const Tensor* branch = with_branch ? &given(args[2], "branch") : nullptr;
     recap_norm_rows_args p;
     std::memset(&p, 0, sizeof(p));

@@ -122,6 +122,8 @@ def test_a_residual_without_a_branch_is_refused():
                dict(), dict(norm=Norm("rms"), out=(x, None))):
         with pytest.raises(ValueError, match="branch must be a tensor"):
             gated_residual(x, None, **kw)
+        with pytest.raises(ValueError, match="branch must be a tensor"):
+            gated_residual(x, False, **kw)
 
 
 def test_forward_mode_tangents_are_refused_not_cut():
