@@ -80,6 +80,16 @@ int type_of(at::ScalarType t, const char* what) {
   refuse(std::string(what) + " must be bfloat16, float16 or float32, not " + c10::toString(t));
 }
 
+// Rows, modulations and parameters are moved 16 bytes at a time.
+bool base_aligned(const Tensor* t) { return t == nullptr || reinterpret_cast<uintptr_t>(t->const_data_ptr()) % 16 == 0; }
+void aligned(const Tensor* t, const char* what) {
+  if (t == nullptr) return;
+  bool good = base_aligned(t);
+  const int64_t unit = 16 / static_cast<int64_t>(t->element_size());
+  for (int64_t i = 0; i + 1 < t->dim(); ++i) good = good && (t->size(i) <= 1 || t->stride(i) % unit == 0);
+  if (!good) refuse(std::string(what) + " must have a base and strides of multiples of 16 bytes");
+}
+
 at::ScalarType dtype_or(PyObject* o, at::ScalarType otherwise) {
   if (o == Py_None) return otherwise;
   if (!THPDtype_Check(o)) refuse("out_dtype must be a dtype");
@@ -114,6 +124,11 @@ struct NormParams {
   const void *weight = nullptr, *bias = nullptr;
   const Tensor* tensors[2] = {nullptr, nullptr};  // weight, bias
   std::optional<Attribute> held[2];
+
+  void check_aligned() const {
+    for (int i = 0; i < 2; ++i)
+      if (!base_aligned(tensors[i])) refuse(std::string("a norm's ") + (i == 0 ? "weight" : "bias") + " must have a base of a multiple of 16 bytes");
+  }
 
   void read(PyObject* norm, int64_t n_head, int64_t n_across, const at::Device& device) {
     {
@@ -387,6 +402,13 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     } else if (k_given != nullptr) {
       refuse("out must match query and key, dim contiguous");
     }
+    if (b != 0 && s != 0) {
+      aligned(&query, "query");
+      aligned(key, "key");
+      aligned(q_given, "the query's out");
+      if (key != nullptr) aligned(k_given, "the key's out");
+      for (const NormParams* n : {&qn, &kn}) n->check_aligned();
+    }
     if (!query.is_cuda()) refuse("rotate_qk runs on CUDA tensors only");
     const c10::cuda::CUDAGuard current(device);
     if (q_given == nullptr) {
@@ -513,6 +535,14 @@ PyObject* norm_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       }
       check_outputs<2>({x_given, h_given}, {&x, with_branch ? branch : &x}, 
                        {&x, branch, mods[0], mods[1], mods[2], n.tensors[0], n.tensors[1], bn.tensors[0], bn.tensors[1]});
+    }
+    if (b != 0 && s != 0) {
+      aligned(&x, with_branch ? "residual" : "x");
+      aligned(branch, "branch");
+      for (int i = 0; i < 3; ++i) aligned(mods[i], names[i]);
+      if (with_branch) aligned(x_given, "the sum's out");
+      aligned(h_given, "the norm's out");
+      for (const NormParams* params : {&n, &bn}) params->check_aligned();
     }
     if (!x.is_cuda()) refuse(std::string(PyUnicode_AsUTF8(args[0])) + " runs on CUDA tensors only");
     const c10::cuda::CUDAGuard current(device);

@@ -156,3 +156,37 @@ def test_foreign_objects_are_refused():
                 call()
         with pytest.raises(ValueError, match="must be an AxialRotary"):
             rotate_qk(q, None, other)
+
+
+def test_misaligned_tensors_are_named():
+    x, w = torch.zeros(2, 3, 16), torch.ones(16)
+    q = torch.zeros(1, 2, 5, 16)
+    odd = lambda t: torch.zeros(t.numel() + 2, dtype=t.dtype)[2:].view(t.shape)  # noqa: E731
+    pitch = torch.zeros(2, 3, 18)[..., :16]  # 72 bytes between rows
+    mods = torch.zeros(2, 3, 18)[..., :16]
+    rms = Norm("rms")
+    for what, call in [
+        ("query must", lambda: rotate_qk(odd(q), None)),
+        ("key must", lambda: rotate_qk(q, odd(q))),
+        ("query's out", lambda: rotate_qk(q, q, out=(odd(q), torch.zeros_like(q)))),
+        ("key's out", lambda: rotate_qk(q, q, out=(torch.zeros_like(q), odd(q)))),
+        ("norm's weight", lambda: rotate_qk(q, None, query_norm=Norm("rms", odd(w)))),
+        ("x must", lambda: modulated_norm(pitch, rms)),
+        ("norm's out", lambda: modulated_norm(x, rms, out=pitch)),
+        ("scale must", lambda: modulated_norm(x, rms, scale=mods)),
+        ("shift must", lambda: modulated_norm(x, rms, shift=odd(w))),
+        ("norm's bias", lambda: modulated_norm(x, Norm("layer", w, odd(w)))),
+        ("residual must", lambda: gated_residual(pitch, x)),
+        ("branch must", lambda: gated_residual(x, pitch)),
+        ("gate must", lambda: gated_residual(x, x, mods)),
+        ("sum's out", lambda: gated_residual(x, x, out=(odd(x), None))),
+    ]:
+        with pytest.raises(ValueError, match=what + ".*16 bytes"):
+            call()
+    with pytest.raises(ValueError, match=CUDA_ONLY):  # contiguous values in any shape
+        modulated_norm(x, Norm("rms", torch.ones(16, 1)))
+    # one row, one vector: strides that take no step do not count
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        modulated_norm(torch.zeros(1, 1, 18)[..., :16], rms, scale=mods[:1, :1])
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        modulated_norm(pitch[:0], rms)
