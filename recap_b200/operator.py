@@ -254,7 +254,11 @@ class Operator:
         """One attention call: ``[b, h, S, d]`` native order in, same shape/dtype out.
 
         With ``rotary`` or the norms, ``query`` and ``key`` are the projections as they come:
-        they are normalised and turned first (``rotate_qk``), in new tensors."""
+        they are normalised and turned first (``rotate_qk``), in new tensors.  A rotary on a grid
+        covers the whole sequence; text that it leaves unturned is the layout's text (a grid
+        without text may run over the joint sequence)."""
+        if rotary is not None:
+            self._check_rotary(rotary, query.shape[-2])
         if not (query.is_cuda and key.is_cuda and value.is_cuda):
             raise ValueError("recap_b200.Operator runs on CUDA tensors only")
         if query.shape != key.shape or key.shape != value.shape:
@@ -275,6 +279,17 @@ class Operator:
         else:
             out = self._refresh(layer, bank, query, key, value)
         return out if in_dtype == torch.bfloat16 else out.to(in_dtype)
+
+    def _check_rotary(self, rotary: AxialRotary, tokens: int) -> None:
+        if not isinstance(rotary, AxialRotary) or rotary.sequence_tokens is None:
+            return
+        if rotary.sequence_tokens != tokens:
+            raise ValueError(f"rotary positions of {rotary.sequence_tokens} tokens for a sequence of {tokens}")
+        text = int(self.layout.text_tokens), bool(self.layout.text_first)
+        if rotary.text_tokens and (rotary.text_tokens, rotary.text_first) != text:
+            side = {True: "first", False: "last"}
+            raise ValueError(f"rotary positions with {rotary.text_tokens} text tokens {side[rotary.text_first]} for a "
+                             f"layout with {text[0]} {side[text[1]]}")
 
     @torch.no_grad()
     def attend_sharded(self, layer_index: int, io) -> None:

@@ -6,7 +6,9 @@ import random
 import pytest
 import torch
 
-from recap_b200 import AxialRotary, Norm, _lib, gated_residual, modulated_norm, rotate_qk
+from recap_b200 import (AxialRotary, HostBankOperator, Norm, Operator, OperatorConfig, _lib, gated_residual,
+                        modulated_norm, rotate_qk)
+from recap_b200.sparse import Layout, SparseGeometry
 
 CUDA_ONLY = "CUDA tensors only"  # what a call that is right but for its device meets
 
@@ -190,3 +192,26 @@ def test_misaligned_tensors_are_named():
         modulated_norm(torch.zeros(1, 1, 18)[..., :16], rms, scale=mods[:1, :1])
     with pytest.raises(ValueError, match=CUDA_ONLY):
         modulated_norm(pitch[:0], rms)
+
+
+@pytest.mark.parametrize("streamed", [False, True])
+def test_attend_refuses_a_rotary_of_another_sequence(streamed):
+    """A longer grid, or text in another place than the layout has it, would turn every token by wrong angles."""
+    layout = Layout.from_permutation(torch.arange(12), text_tokens=5, text_first=True)
+    cls = HostBankOperator if streamed else Operator
+    op = cls.build(OperatorConfig(), SparseGeometry.build(layout, 128), n_layers=1)
+    q = torch.zeros(1, 2, 17, 16)
+    turn = lambda grid, **kw: op.attend(0, q, q, q, rotary=AxialRotary(16, (8, 8), grid=grid, **kw))  # noqa: E731
+    with pytest.raises(ValueError, match="24 tokens for a sequence of 17"):
+        turn((4, 6))
+    with pytest.raises(ValueError, match="21 tokens for a sequence of 17"):
+        turn((4, 4), text_tokens=5, text_first=True)
+    with pytest.raises(ValueError, match="16 tokens for a sequence of 17"):
+        turn((4, 4))
+    with pytest.raises(ValueError, match="5 text tokens last .* with 5 first"):
+        turn((3, 4), text_tokens=5)
+    with pytest.raises(ValueError, match="7 text tokens first .* with 5 first"):
+        turn((2, 5), text_tokens=7, text_first=True)
+    for right in (dict(grid=(3, 4), text_tokens=5, text_first=True), dict(grid=(17, 1)), dict(grid=None)):
+        with pytest.raises(ValueError, match=CUDA_ONLY):
+            turn(right.pop("grid"), **right)
