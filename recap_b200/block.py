@@ -116,8 +116,8 @@ class AxialRotary:
         else:
             turns = [theta ** -(2.0 * i / d) / (2.0 * math.pi) for theta, d in zip(thetas, dims) for i in range(d // 2)]
         axis = [a for a, d in enumerate(dims) for _ in range(d // 2)]
-        # turns for each unit of position, as 64 bits of a turn
-        c.turns[:len(turns)] = [round(f * scales[a] % 1.0 * 2.0**64) % 2**64 for f, a in zip(turns, axis)]
+        # turns for each unit of position, as 64 bits of a turn; fmod keeps the sign, and with it the bits of small negative ones
+        c.turns[:len(turns)] = [round(math.fmod(f * scales[a], 1.0) * 2.0**64) % 2**64 for f, a in zip(turns, axis)]
         if any(starts):
             # added to the top 32 bits of the product, which are cut: up makes up for down
             c.phase[:len(turns)] = [math.ceil(f * starts[a] % 1.0 * 2.0**32) % 2**32 << 32 for f, a in zip(turns, axis)]
