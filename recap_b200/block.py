@@ -67,7 +67,9 @@ class AxialRotary:
     the grid coordinates of the token index, and the ``text_tokens`` before (``text_first``)
     or after the grid are not turned: the native token order of ``Layout``.  Without it the
     positions come with each call as an integer tensor, of any size: angles are kept as
-    64-bit fractions of a turn, so a far position turns as exactly as a near one.
+    64-bit fractions of a turn and wrap without rounding.  The frequencies are doubles, as models
+    form them: an angle is within 2^-32 + |position * scale| 2^-53 of a turn of the definition's (theta
+    of 1 or more), that is within 2^-31 up to positions of 2^21, 2^-22 up to 2^31.
 
     The object holds numbers on the host only: it serves every device, stream and graph.
     """
