@@ -428,9 +428,11 @@ int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
   const unsigned blocks = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.blocks);
   const int block = kWarps ? 32 * kTeams : threads;
   int smem = 0;
-  if (stages<TX, kVec, kRows, kGate>()) {
-    smem = kRows * kVec * (slots_of(sizeof(TX)) + (kGate && sizeof(TH) == sizeof(TX) ? slots_of(sizeof(TH)) : 0)) * block * 16;
-    if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if constexpr (stages<TX, kVec, kRows, kGate>()) {
+    constexpr int kPerThread = kRows * kVec * (slots_of(sizeof(TX)) + (kGate && sizeof(TH) == sizeof(TX) ? slots_of(sizeof(TH)) : 0)) * 16;
+    smem = kPerThread * block;
+    // the most of any call, so that calls of two host threads set the same
+    if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPerThread * kThreads) != cudaSuccess)
       return kErrLaunch;
   }
   return launch_after(kernel, dim3(blocks), block, smem, s, a);

@@ -487,7 +487,9 @@ template <typename TI, typename TO, int kLanes, int kNorm, bool kHalves>
 int launch_kernel(const RotateArgs& a, dim3 grid, int smem, cudaStream_t s) {
   if constexpr (kNorm == kNormRmsAcross) {
     auto* kernel = rotate_across_kernel<TI, TO, kLanes, kHalves>;
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    // the most of any call, so that calls of two host threads set the same: rows of a group and the weights of all heads
+    constexpr int kMost = kAcrossRows * kThreads * (sizeof(TI) == 4 ? 32 : 16) + kThreads / kLanes * kAcrossHeads * 2 * kLanes * 16;
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess)
       return kErrLaunch;
     return launch_after(kernel, grid, kThreads, smem, s, a);
   } else {
