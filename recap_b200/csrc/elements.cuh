@@ -31,6 +31,14 @@ int launch_after(void (*kernel)(Args), dim3 grid, int threads, int smem, cudaStr
   return kErrLaunch;
 }
 
+// Lets a kernel's blocks have `bytes` of dynamic shared memory.
+template <typename Args>
+bool allow_shared(void (*kernel)(Args), int bytes) {
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) return true;
+  cudaGetLastError();  // as above
+  return false;
+}
+
 // Two 16-bit values of a 32-bit word <-> fp32 (bf16 widens by a shift; fp16 converts).
 template <typename T>
 __device__ __forceinline__ float2 unpack2(uint32_t w);

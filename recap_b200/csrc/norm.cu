@@ -432,8 +432,7 @@ int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
     constexpr int kPerThread = kRows * kVec * (slots_of(sizeof(TX)) + (kGate && sizeof(TH) == sizeof(TX) ? slots_of(sizeof(TH)) : 0)) * 16;
     smem = kPerThread * block;
     // the most of any call, so that calls of two host threads set the same
-    if (smem > 46 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kPerThread * kThreads) != cudaSuccess)
-      return kErrLaunch;
+    if (smem > 46 * 1024 && !allow_shared(kernel, kPerThread * kThreads)) return kErrLaunch;
   }
   return launch_after(kernel, dim3(blocks), block, smem, s, a);
 }

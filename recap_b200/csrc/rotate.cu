@@ -489,8 +489,7 @@ int launch_kernel(const RotateArgs& a, dim3 grid, int smem, cudaStream_t s) {
     auto* kernel = rotate_across_kernel<TI, TO, kLanes, kHalves>;
     // the most of any call, so that calls of two host threads set the same: rows of a group and the weights of all heads
     constexpr int kMost = kAcrossRows * kThreads * (sizeof(TI) == 4 ? 32 : 16) + kThreads / kLanes * kAcrossHeads * 2 * kLanes * 16;
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess)
-      return kErrLaunch;
+    if (smem > 40 * 1024 && !allow_shared(kernel, kMost)) return kErrLaunch;
     return launch_after(kernel, grid, kThreads, smem, s, a);
   } else {
     return launch_after(rotate_kernel<TI, TO, kLanes, kNorm, kHalves>, grid, kThreads, 0, s, a);
