@@ -437,10 +437,11 @@ int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
   return launch_after(kernel, dim3(blocks), block, smem, s, a);
 }
 
-template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads>
+// kOneWarp: rows of 32 threads come here too.
+template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, int kThreads, bool kOneWarp = kVec == 1>
 int launch_team(NormArgs& a, int threads, cudaStream_t s) {
   // a row of one warp leaves a block room for others'
-  if constexpr (kVec == 1)
+  if constexpr (kOneWarp)
     if (threads == 32) return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, 32 * kTeams, true, false>(a, threads, s);
   if (a.C == 8 * kVec * threads) return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, false, true>(a, threads, s);
   return launch_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, false, false>(a, threads, s);
@@ -454,10 +455,14 @@ int launch_team(NormArgs& a, int threads, cudaStream_t s) {
 template <typename TX, typename TH, int kVec, int kRows, int kMods, int kThreads = 512>
 int launch_gate(NormArgs& a, int threads, cudaStream_t s) {
   if (a.branch == nullptr) return launch_team<TX, TH, kVec, kRows, false, kMods, kThreads>(a, threads, s);
-  if constexpr (kRows == 4 && sizeof(TX) == 4) {
-    if (sizeof(TH) == 4 || threads <= 320) return launch_team<TX, TH, kVec, 2, true, kMods, kThreads>(a, threads, s);
+  if constexpr (kRows == 4 && sizeof(TX) == 4 && sizeof(TH) == 4) {
+    return launch_team<TX, TH, kVec, 2, true, kMods, kThreads>(a, threads, s);
+  } else if constexpr (kRows == 4 && sizeof(TX) == 4) {
+    if (threads <= 320) return launch_team<TX, TH, kVec, 2, true, kMods, kThreads>(a, threads, s);
+    return launch_team<TX, TH, kVec, kRows, true, kMods, kThreads, false>(a, threads, s);
+  } else {
+    return launch_team<TX, TH, kVec, kRows, true, kMods, kThreads>(a, threads, s);
   }
-  return launch_team<TX, TH, kVec, kRows, true, kMods, kThreads>(a, threads, s);
 }
 
 template <typename TX, typename TH>
@@ -481,8 +486,10 @@ int launch_vec(NormArgs& a, cudaStream_t s) {
     if (!many) return launch_gate<TX, TH, 1, 1, kMods16>(a, threads, s);
     // two tokens and their modulations in 80 registers rather than 64 as long as blocks are small enough
     // (2304 values, both norms, bf16: 87 us, in 64 registers 90 us)
-    if (threads <= 384) return launch_gate<TX, TH, 1, 2, kMods16, 384>(a, threads, s);
-    return launch_gate<TX, TH, 1, 2, kMods16>(a, threads, s);
+    if constexpr (one_vector_threads(sizeof(TX)) > 384) {
+      if (threads > 384) return launch_gate<TX, TH, 1, 2, kMods16>(a, threads, s);
+    }
+    return launch_gate<TX, TH, 1, 2, kMods16, 384>(a, threads, s);
   }
   if (per == 2) {
     if constexpr (sizeof(TX) == 2) {
