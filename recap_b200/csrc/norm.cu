@@ -424,7 +424,7 @@ template <typename TX, typename TH, int kVec, int kRows, bool kGate, int kMods, 
 int launch_kernel(NormArgs& a, int threads, cudaStream_t s) {
   auto* kernel = norm_kernel<TX, TH, kVec, kRows, kGate, kMods, kThreads, kWarps, kWhole>;
   constexpr int kTokens = kRows * (kWarps ? kTeams : 1);  // of a block
-  a.blocks = (a.S + kTokens - 1) / kTokens;
+  a.blocks = (a.S - 1) / kTokens + 1;  // S up to 2^31 - 1
   const unsigned blocks = static_cast<unsigned>(a.batch) * static_cast<unsigned>(a.blocks);
   const int block = kWarps ? 32 * kTeams : threads;
   int smem = 0;

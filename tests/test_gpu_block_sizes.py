@@ -1,0 +1,29 @@
+"""The operators around the attention at the largest sizes that they take."""
+
+import pytest
+import torch
+
+from recap_b200 import Norm, gated_residual, modulated_norm
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+BF = torch.bfloat16
+
+
+def _needs(gigabytes):
+    if torch.cuda.mem_get_info()[0] < gigabytes * 2**30:
+        pytest.skip(f"needs {gigabytes} GB")
+
+
+@pytest.mark.parametrize("gated", [False, True])
+def test_most_tokens(gated):
+    """2^31 - 1 tokens of eight channels, all of them one row: each output row is that row's."""
+    _needs(48)
+    tokens = 2**31 - 1
+    row = torch.randn(1, 8, device=DEV).to(BF)
+    x = row.expand(tokens, 8)
+    want = gated_residual(row, row)[0] if gated else modulated_norm(row, Norm("rms"))
+    got = gated_residual(x, x)[0] if gated else modulated_norm(x, Norm("rms"))
+    for lo in range(0, tokens, 2**28):
+        assert bool((got[lo:lo + 2**28] == want).all())
