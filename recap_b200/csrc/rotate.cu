@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
   // the group's rows are heads slot, slot + split, ...: `mine` of them (none for a lane past the row or a
   // group past the tokens), `most` in any group
   const int heads = a.heads[t];
-  const int most = (heads + me.split - 1) >> me.log2;
-  const int mine = me.active ? (heads - me.slot + me.split - 1) >> me.log2 : 0;
+  const int most = ((heads - 1) >> me.log2) + 1;
+  const int mine = me.active ? ((heads - me.slot - 1) >> me.log2) + 1 : 0;
   const TI* src = static_cast<const TI*>(a.x[t]) + me.b * a.x_stride[t][0] + me.s * a.x_stride[t][2] +
                   (me.slot < heads ? me.slot : 0) * a.x_stride[t][1];
   // Every group has the same rows, in whole batches: nothing to ask for row by row, in the layer norm of 16-bit rows,
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_across_kernel(const __grid
   const int d0 = me.d0, d1 = me.d1;
   const int t = blockIdx.y;
   const int heads = a.heads[t];
-  const int mine = me.active ? (heads - me.slot + me.split - 1) >> me.log2 : 0;
+  const int mine = me.active ? ((heads - me.slot - 1) >> me.log2) + 1 : 0;
   const bool weighted = a.weight[t] != nullptr;
   float4* weights = reinterpret_cast<float4*>(s_dynamic) + me.lane;
   uint4* rows = s_dynamic + (weighted ? heads * (2 * kLanes) : 0) + threadIdx.x;
@@ -555,9 +555,9 @@ int launch_rotate(RotateArgs& a, cudaStream_t s) {
   int log2 = 0;
   int64_t least = -1;
   for (int l = 0; (1 << l) <= groups && (l == 0 || (1 << (l - 1)) < most); ++l) {
-    const int rows = (most + (1 << l) - 1) >> l;
+    const int rows = ((most - 1) >> l) + 1;
     if (across && rows > kAcrossRows && (2 << l) <= groups) continue;
-    const int64_t cost = (blocks(l) * tensors + resident - 1) / resident * (80 * rows + 330);
+    const int64_t cost = (blocks(l) * tensors + resident - 1) / resident * (80LL * rows + 330);
     if (least < 0 || cost < least) {
       least = cost;
       log2 = l;
@@ -569,7 +569,7 @@ int launch_rotate(RotateArgs& a, cudaStream_t s) {
   int smem = 0;
   if (across) {
     const bool weighted = a.weight[0] != nullptr || a.weight[1] != nullptr;
-    const int rows = (most + (1 << log2) - 1) >> log2;
+    const int rows = ((most - 1) >> log2) + 1;
     smem = rows * kThreads * (a.in_type == kTypeF32 ? 32 : 16) + (weighted ? most * 2 * lanes * 16 : 0);
   }
   if (a.in_type == kTypeBf16 && a.out_type == kTypeBf16)

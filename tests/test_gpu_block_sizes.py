@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from recap_b200 import Norm, gated_residual, modulated_norm
+from recap_b200 import Norm, gated_residual, modulated_norm, rotate_qk
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,13 @@ def test_most_tokens(gated):
     got = gated_residual(x, x)[0] if gated else modulated_norm(x, Norm("rms"))
     for lo in range(0, tokens, 2**28):
         assert bool((got[lo:lo + 2**28] == want).all())
+
+
+@pytest.mark.parametrize("heads", [2**25 + 1, 2**27 - 3])
+def test_many_heads(heads):
+    """Heads whose cost, counted in instructions, passes 2^31."""
+    _needs(8)
+    row = torch.randn(1, 1, 1, 8, device=DEV).to(BF)
+    norm = Norm("rms")
+    want = rotate_qk(row, None, query_norm=norm)[0]
+    assert bool((rotate_qk(row.expand(1, heads, 1, 8), None, query_norm=norm)[0] == want).all())
