@@ -126,7 +126,7 @@ def native():
         try:
             from . import _native as module
         except ImportError as error:
-            raise RuntimeError("_native.so is not built; run `python -m recap_b200.build`") from error
+            raise RuntimeError("_native.so is not built, or for another Python or torch; run `python -m recap_b200.build`") from error
         module.bind(*(ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in ("recap_rotate_qk", "recap_norm_rows")),
                     check)
         _native = module

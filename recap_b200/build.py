@@ -63,20 +63,37 @@ def _stale() -> bool:
     return any(p.stat().st_mtime > built for p in inputs)
 
 
-def _start_binding(force: bool) -> subprocess.Popen | None:
-    """Start compiling the binding if it is out of date."""
-    inputs = [BINDING, INCLUDE / "recap_b200.h", Path(__file__)]
-    if not force and BINDING_PATH.exists() and all(p.stat().st_mtime <= BINDING_PATH.stat().st_mtime for p in inputs):
-        return None
+def _binding_command() -> list[str]:
+    """The compiler call of the binding, for the running Python and its torch."""
     import torch
 
     root = Path(torch.__file__).resolve().parent
-    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
-           f"-I{root / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
-           f"-I{Path(_cuda_home()) / 'include'}", str(BINDING), "-o", str(BINDING_PATH.with_suffix(".so.tmp")),
-           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
-    return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{root / 'include'}",
+            f"-I{root / 'include/torch/csrc/api/include'}", f"-I{sysconfig.get_paths()['include']}",
+            f"-I{Path(_cuda_home()) / 'include'}", str(BINDING), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu",
+            "-ltorch_python"]
+
+
+def _binding_stamp() -> str:
+    """What a built binding belongs to, kept beside it: it loads into this Python and torch only."""
+    import torch
+
+    return f"python {sys.version_info[0]}.{sys.version_info[1]} {sysconfig.get_config_var('SOABI')}, torch {torch.__version__}\n"
+
+
+def _binding_sources_newer() -> bool:
+    inputs = [BINDING, INCLUDE / "recap_b200.h", Path(__file__)]
+    return not BINDING_PATH.exists() or any(p.stat().st_mtime > BINDING_PATH.stat().st_mtime for p in inputs)
+
+
+def _start_binding(force: bool) -> subprocess.Popen | None:
+    """Start compiling the binding if it is out of date."""
+    stamp = BINDING_PATH.with_suffix(".txt")
+    if not force and not _binding_sources_newer() and stamp.exists() and stamp.read_text() == _binding_stamp():
+        return None
+    return subprocess.Popen([*_binding_command(), "-o", str(BINDING_PATH.with_suffix(".so.tmp"))], stdout=subprocess.PIPE,
+                            stderr=subprocess.STDOUT, text=True)
 
 
 def _finish_binding(process: subprocess.Popen | None) -> None:
@@ -84,17 +101,33 @@ def _finish_binding(process: subprocess.Popen | None) -> None:
         return
     out, _ = process.communicate()
     if process.returncode != 0:
-        raise RuntimeError("the binding did not compile:\n" + out)
+        raise RuntimeError(out)
     os.replace(BINDING_PATH.with_suffix(".so.tmp"), BINDING_PATH)
+    BINDING_PATH.with_suffix(".txt").write_text(_binding_stamp())
 
 
 def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile the binding and every kernel source and link the shared library; returns its path."""
-    binding = _start_binding(force)
+    """Compile the binding and every kernel source and link the shared library; returns its path.
+    The library needs nothing of the binding: where that does not compile (no host compiler, no headers of
+    Python or torch), this says so on stderr, and the row kernels raise when they are called from Python."""
+    binding, error = None, None
     try:
-        return _build_library(force, verbose)
+        binding = _start_binding(force)
+    except (ImportError, OSError) as e:
+        error = e
+    try:
+        path = _build_library(force, verbose)
     finally:
-        _finish_binding(binding)
+        try:
+            _finish_binding(binding)
+        except RuntimeError as e:
+            error = e
+    if error is not None:
+        if _binding_sources_newer():
+            BINDING_PATH.unlink(missing_ok=True)  # one of older sources would not fit the library
+        print(f"the binding of the row kernels ({BINDING_PATH.name}) was not built; the library and all that does not call "
+              f"them do without it: {error}", file=sys.stderr)
+    return path
 
 
 def _build_library(force: bool, verbose: bool) -> Path:
