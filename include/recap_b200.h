@@ -353,7 +353,7 @@ typedef struct recap_rotary {
  * element strides (b, h, s) in strides[0 .. 2] and [3 .. 5]; q_out and k_out likewise with strides
  * [6 .. 8] and [9 .. 11]; k and k_out NULL with k_heads 0.  An output may be its input; otherwise
  * it must not overlap either input.  Every base is 16-byte aligned, every stride a multiple of 16
- * bytes, D a multiple of 8 up to 256.  out_type is in_type or bf16.
+ * bytes, D a multiple of 8 up to 256, at most 2^31 - 32 heads.  out_type is in_type or bf16.
  *   positions       int32 or int64 (position_bits 32 or 64) [batch, S, axes] with element strides
  *                   position_strides (b, s, axis), or NULL with position_bits 0 (grid, or no turn)
  *   first_token     the place in the grid's sequence of token 0 of this call

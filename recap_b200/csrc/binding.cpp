@@ -327,7 +327,7 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
       if (key->scalar_type() != query.scalar_type() || key->device() != device) refuse("query and key differ in dtype or device");
       if (hk < 1) refuse("key has no heads");
     }
-    if (b * s > 0x7fffffff || std::max(hq, hk) > 0x7fffffff) refuse("more than 2^31 - 1 tokens or heads");
+    if (b * s > 0x7fffffff || std::max(hq, hk) > 0x7fffffff - 31) refuse("more than 2^31 - 1 tokens or 2^31 - 32 heads");
     no_gradient(&query);
     no_gradient(key);
     p.in_type = type_of(query.scalar_type(), "query");

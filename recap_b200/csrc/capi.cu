@@ -704,7 +704,7 @@ extern "C" {
 
 int recap_rotate_qk(const recap_rotate_qk_args* p, const recap_rotary* rotary, void* stream) {
   if (p == nullptr || p->batch < 0 || p->S < 0 || p->q_heads <= 0 || p->k_heads < 0 || p->D <= 0 || p->D > 256 ||
-      p->D % 8 || p->norm < kNormNone || p->norm > kNormRmsAcross || !type_ok(p->in_type) || !type_ok(p->weight_type))
+      p->q_heads > rotate_max_heads() || p->k_heads > rotate_max_heads() || p->D % 8 || p->norm < kNormNone || p->norm > kNormRmsAcross || !type_ok(p->in_type) || !type_ok(p->weight_type))
     return kErrShape;
   if (p->out_type != p->in_type && p->out_type != kTypeBf16) return kErrUnsupported;
   if (p->norm == kNormRmsAcross &&

@@ -274,6 +274,7 @@ struct RotateArgs {
   uint64_t phase[kMaxPairs];
   uint8_t axis[kMaxPairs];
 };
+int rotate_max_heads();
 int rotate_max_heads_across(int D);
 int launch_rotate(RotateArgs& a, cudaStream_t s);
 

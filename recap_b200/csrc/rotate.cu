@@ -233,8 +233,8 @@ __global__ void __launch_bounds__(kThreads, sizeof(TI) == 4 ? 3 : 4)
   // the group's rows are heads slot, slot + split, ...: `mine` of them (none for a lane past the row or a
   // group past the tokens), `most` in any group
   const int heads = a.heads[t];
-  const int most = ((heads - 1) >> me.log2) + 1;
-  const int mine = me.active ? ((heads - me.slot - 1) >> me.log2) + 1 : 0;
+  const int most = (heads + me.split - 1) >> me.log2;
+  const int mine = me.active ? (heads - me.slot + me.split - 1) >> me.log2 : 0;
   const TI* src = static_cast<const TI*>(a.x[t]) + me.b * a.x_stride[t][0] + me.s * a.x_stride[t][2] +
                   (me.slot < heads ? me.slot : 0) * a.x_stride[t][1];
   // Every group has the same rows, in whole batches: nothing to ask for row by row, in the layer norm of 16-bit rows,
@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 4) rotate_across_kernel(const __grid
   const int d0 = me.d0, d1 = me.d1;
   const int t = blockIdx.y;
   const int heads = a.heads[t];
-  const int mine = me.active ? ((heads - me.slot - 1) >> me.log2) + 1 : 0;
+  const int mine = me.active ? (heads - me.slot + me.split - 1) >> me.log2 : 0;
   const bool weighted = a.weight[t] != nullptr;
   float4* weights = reinterpret_cast<float4*>(s_dynamic) + me.lane;
   uint4* rows = s_dynamic + (weighted ? heads * (2 * kLanes) : 0) + threadIdx.x;
@@ -529,6 +529,9 @@ Divisor divisor(uint32_t d) {
 }
 
 }  // namespace
+
+// Heads and a group's split less one are added in 32 bits.
+int rotate_max_heads() { return 0x7fffffff - (kThreads / 8 - 1); }
 
 int rotate_max_heads_across(int D) { return kThreads / (D <= 64 ? 8 : D <= 128 ? 16 : 32) * kAcrossHeads; }
 

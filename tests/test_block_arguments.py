@@ -215,3 +215,18 @@ def test_attend_refuses_a_rotary_of_another_sequence(streamed):
     for right in (dict(grid=(3, 4), text_tokens=5, text_first=True), dict(grid=(17, 1)), dict(grid=None)):
         with pytest.raises(ValueError, match=CUDA_ONLY):
             turn(right.pop("grid"), **right)
+
+
+def test_more_heads_than_32_bits_count_are_refused():
+    row = torch.zeros(1, 1, 1, 8)
+    for heads in (2**31 - 31, 2**31 - 1, 2**31):
+        with pytest.raises(ValueError, match="heads"):
+            rotate_qk(row.expand(1, heads, 1, 8), None)
+    with pytest.raises(ValueError, match=CUDA_ONLY):
+        rotate_qk(row.expand(1, 2**31 - 32, 1, 8), None)
+    import struct
+
+    args = lambda hq, hk: struct.Struct("<4Q12qQ3qq4Q10i2f").pack(  # noqa: E731
+        4096, 8192, 4096, 8192, *[8] * 12, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, hq, hk, 1, 8, 0, 0, 0, 0, 0, 1e-6, 1e-6)
+    for hq, hk in ((2**31 - 31, 1), (1, 2**31 - 1)):
+        assert _lib.load().recap_rotate_qk(args(hq, hk), None, None) == _lib.RECAP_ERR_SHAPE
