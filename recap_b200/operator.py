@@ -254,9 +254,9 @@ class Operator:
         """One attention call: ``[b, h, S, d]`` native order in, same shape/dtype out.
 
         With ``rotary`` or the norms, ``query`` and ``key`` are the projections as they come:
-        they are normalised and turned first (``rotate_qk``), in new tensors.  A rotary on a grid
-        covers the whole sequence; text that it leaves unturned is the layout's text (a grid
-        without text may run over the joint sequence)."""
+        they are normalised and turned first (``rotate_qk``), in new tensors.  The grid of a
+        rotary is the layout's video, at its place in the sequence (text behind it may be shorter
+        than the rotary's), or, without text, runs over the joint sequence."""
         if rotary is not None:
             self._check_rotary(rotary, query.shape[-2])
         if not (query.is_cuda and key.is_cuda and value.is_cuda):
@@ -283,13 +283,13 @@ class Operator:
     def _check_rotary(self, rotary: AxialRotary, tokens: int) -> None:
         if not isinstance(rotary, AxialRotary) or rotary.sequence_tokens is None:
             return
-        if rotary.sequence_tokens != tokens:
-            raise ValueError(f"rotary positions of {rotary.sequence_tokens} tokens for a sequence of {tokens}")
-        text = int(self.layout.text_tokens), bool(self.layout.text_first)
-        if rotary.text_tokens and (rotary.text_tokens, rotary.text_first) != text:
-            side = {True: "first", False: "last"}
-            raise ValueError(f"rotary positions with {rotary.text_tokens} text tokens {side[rotary.text_first]} for a "
-                             f"layout with {text[0]} {side[text[1]]}")
+        if not rotary.text_tokens and rotary.sequence_tokens == tokens:
+            return
+        video = rotary.sequence_tokens - rotary.text_tokens, rotary.text_tokens if rotary.text_first else 0
+        mine = int(self.layout.video_tokens), video_offset(self.layout)
+        if video != mine or rotary.sequence_tokens < tokens:
+            raise ValueError(f"rotary positions of {rotary.sequence_tokens} tokens, {video[0]} of them video from {video[1]} on, "
+                             f"for a sequence of {tokens} with {mine[0]} from {mine[1]} on")
 
     @torch.no_grad()
     def attend_sharded(self, layer_index: int, io) -> None:

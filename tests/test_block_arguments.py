@@ -202,19 +202,26 @@ def test_attend_refuses_a_rotary_of_another_sequence(streamed):
     op = cls.build(OperatorConfig(), SparseGeometry.build(layout, 128), n_layers=1)
     q = torch.zeros(1, 2, 17, 16)
     turn = lambda grid, **kw: op.attend(0, q, q, q, rotary=AxialRotary(16, (8, 8), grid=grid, **kw))  # noqa: E731
-    with pytest.raises(ValueError, match="24 tokens for a sequence of 17"):
-        turn((4, 6))
-    with pytest.raises(ValueError, match="21 tokens for a sequence of 17"):
-        turn((4, 4), text_tokens=5, text_first=True)
-    with pytest.raises(ValueError, match="16 tokens for a sequence of 17"):
-        turn((4, 4))
-    with pytest.raises(ValueError, match="5 text tokens last .* with 5 first"):
-        turn((3, 4), text_tokens=5)
-    with pytest.raises(ValueError, match="7 text tokens first .* with 5 first"):
-        turn((2, 5), text_tokens=7, text_first=True)
+    for grid, kw in (((4, 6), {}), ((4, 4), dict(text_tokens=5, text_first=True)), ((4, 4), {}), ((3, 4), dict(text_tokens=5)),
+                     ((2, 5), dict(text_tokens=7, text_first=True)), ((3, 4), dict(text_tokens=6, text_first=True))):
+        with pytest.raises(ValueError, match="rotary positions of .* for a sequence of 17 with 12 from 5 on"):
+            turn(grid, **kw)
     for right in (dict(grid=(3, 4), text_tokens=5, text_first=True), dict(grid=(17, 1)), dict(grid=None)):
         with pytest.raises(ValueError, match=CUDA_ONLY):
             turn(right.pop("grid"), **right)
+
+
+def test_attend_takes_a_rotary_with_room_for_longer_text():
+    """Text behind the video does not move it: a rotary for the longest text serves shorter ones."""
+    layout = Layout.from_permutation(torch.arange(12), text_tokens=5, text_first=False)
+    op = Operator.build(OperatorConfig(), SparseGeometry.build(layout, 128), n_layers=1)
+    q = torch.zeros(1, 2, 17, 16)
+    for text in (5, 9, 200):
+        with pytest.raises(ValueError, match=CUDA_ONLY):
+            op.attend(0, q, q, q, rotary=AxialRotary(16, (8, 8), grid=(3, 4), text_tokens=text))
+    for text, first in ((4, False), (0, False), (5, True)):
+        with pytest.raises(ValueError, match="for a sequence of 17 with 12 from 0 on"):
+            op.attend(0, q, q, q, rotary=AxialRotary(16, (8, 8), grid=(3, 4), text_tokens=text, text_first=first))
 
 
 def test_more_heads_than_32_bits_count_are_refused():
