@@ -351,8 +351,8 @@ typedef struct recap_rotary {
 
 /* Operands of recap_rotate_qk (host struct).  q and k [batch, heads, S, D] with D contiguous and
  * element strides (b, h, s) in strides[0 .. 2] and [3 .. 5]; q_out and k_out likewise with strides
- * [6 .. 8] and [9 .. 11]; k and k_out NULL with k_heads 0.  An output may be its input; otherwise
- * it must not overlap either input.  Every base is 16-byte aligned, every stride a multiple of 16
+ * [6 .. 8] and [9 .. 11]; k and k_out NULL with k_heads 0.  An output may be its own input; otherwise
+ * it must not overlap either input, the parameters or the positions.  Every base is 16-byte aligned, every stride a multiple of 16
  * bytes, D a multiple of 8 up to 256, at most 2^31 - 32 heads.  out_type is in_type or bf16.
  *   positions       int32 or int64 (position_bits 32 or 64) [batch, S, axes] with element strides
  *                   position_strides (b, s, axis), or NULL with position_bits 0 (grid, or no turn)
@@ -380,8 +380,8 @@ int recap_rotate_qk(const recap_rotate_qk_args* args, const recap_rotary* rotary
 /* Operands of recap_norm_rows (host struct).  x [batch, S, C] of x_type; branch (nullable) and h of
  * h_type, which is x_type or, for fp32 x, bf16 or fp16; x_out of x_type.  C contiguous, a multiple of 8
  * up to 16384; element strides (b, s): strides[0 .. 1] x, [2 .. 3] branch, [4 .. 5] x_out, [6 .. 7] h,
- * multiples of 16 bytes, bases 16-byte aligned.  An output may be its input of the same type; otherwise
- * it must not overlap an input.
+ * multiples of 16 bytes, bases 16-byte aligned.  x_out may be x, and h the branch (without
+ * one, x), of one type; otherwise an output must not overlap an input, scale, shift and the parameters among them.
  *   scale, shift, gate  of mod_type (nullable each) with element strides (b, s) in mod_strides
  *                       [0 .. 1], [2 .. 3], [4 .. 5]; 0 where one vector serves every sample or token
  *   weight, bias, branch_weight, branch_bias  [C] (nullable each) of weight_type, branch_weight_type

@@ -229,21 +229,21 @@ bool same(const Tensor& x, const Tensor& y) {
   return x.const_data_ptr() == y.const_data_ptr() && x.scalar_type() == y.scalar_type();
 }
 
-// Outputs hold each element once (distinct()), may be the input of the same place in the list, and otherwise
-// overlap neither an input nor one another.
-template <size_t N>
-void check_outputs(const std::array<const Tensor*, N>& outs, const std::array<const Tensor*, N>& own,
-                   std::initializer_list<const Tensor*> inputs) {
-  for (size_t i = 0; i < N; ++i) {
-    const Tensor* o = outs[i];
-    if (o == nullptr) continue;
-    if (o->numel() != 0 && !distinct(*o)) refuse("an output holds an element twice (an expanded tensor, or strides within one another)");
-    for (const Tensor* x : inputs)
-      if (x != nullptr && !(x == own[i] && same(*o, *x)) && !apart(*o, *x))
-        refuse("an output overlaps an input (it may only be that input itself)");
-    for (size_t j = i + 1; j < N; ++j)
-      if (outs[j] != nullptr && !apart(*o, *outs[j])) refuse("the outputs overlap");
-  }
+// An output holds each element once and overlaps none of `inputs`, but for `own`, the input that it may replace: every element
+// of that is read by the thread that writes it, before it does, also where the call has it in another of these places.
+void check_output(const Tensor* o, const Tensor* own, std::initializer_list<const Tensor*> inputs) {
+  if (o == nullptr) return;
+  if (o->numel() != 0 && !distinct(*o)) refuse("an output holds an element twice (an expanded tensor, or strides within one another)");
+  for (const Tensor* x : inputs)
+    if (x != nullptr && !(x == own && same(*o, *x)) && !apart(*o, *x))
+      refuse("an output overlaps an input (it may only be that input itself)");
+}
+
+// Nor may it overlap what other threads read, or this one after the output is written.
+void check_clear(const Tensor* o, std::initializer_list<const Tensor*> inputs) {
+  if (o == nullptr) return;
+  for (const Tensor* x : inputs)
+    if (x != nullptr && !apart(*o, *x)) refuse("an output overlaps an input that is read beside it");
 }
 
 Tensor allocate(const Tensor& like, at::ScalarType dtype) {
@@ -397,8 +397,12 @@ PyObject* rotate_qk(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         if (o->scalar_type() != out_dtype) refuse("out differs in dtype");
         no_gradient(o);
       }
-      check_outputs<2>({q_given, key != nullptr ? k_given : nullptr}, {&query, key},
-                       {&query, key, qn.tensors[0], qn.tensors[1], kn.tensors[0], kn.tensors[1], positions});
+      const Tensor* k_to = key != nullptr ? k_given : nullptr;
+      check_output(q_given, &query, {&query});
+      check_output(k_to, key, {key});
+      // query and key are turned by different blocks
+      check_clear(q_given, {key, k_to, qn.tensors[0], qn.tensors[1], kn.tensors[0], kn.tensors[1], positions});
+      check_clear(k_to, {&query, qn.tensors[0], qn.tensors[1], kn.tensors[0], kn.tensors[1], positions});
     } else if (k_given != nullptr) {
       refuse("out must match query and key, dim contiguous");
     }
@@ -533,8 +537,11 @@ PyObject* norm_rows(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         if (h_given->scalar_type() != h_dtype) refuse("the norm's out differs in dtype");
         rows(*h_given, "out", ignored);
       }
-      check_outputs<2>({x_given, h_given}, {&x, with_branch ? branch : &x}, 
-                       {&x, branch, mods[0], mods[1], mods[2], n.tensors[0], n.tensors[1], bn.tensors[0], bn.tensors[1]});
+      check_output(x_given, &x, {&x, branch, mods[2]});
+      check_output(h_given, with_branch ? branch : &x, {&x, branch, mods[0], mods[1], mods[2]});
+      // the sum is stored before the norm's modulations are read
+      check_clear(x_given, {h_given, mods[0], mods[1], n.tensors[0], n.tensors[1], bn.tensors[0], bn.tensors[1]});
+      check_clear(h_given, {n.tensors[0], n.tensors[1], bn.tensors[0], bn.tensors[1]});
     }
     if (b != 0 && s != 0) {
       aligned(&x, with_branch ? "residual" : "x");

@@ -237,3 +237,25 @@ def test_more_heads_than_32_bits_count_are_refused():
         4096, 8192, 4096, 8192, *[8] * 12, 0, 0, 0, 0, 0, 0, 0, 0, 0, 1, hq, hk, 1, 8, 0, 0, 0, 0, 0, 1e-6, 1e-6)
     for hq, hk in ((2**31 - 31, 1), (1, 2**31 - 1)):
         assert _lib.load().recap_rotate_qk(args(hq, hk), None, None) == _lib.RECAP_ERR_SHAPE
+
+
+def test_one_tensor_in_two_places_with_an_output_over_it():
+    """Query and key are turned by different blocks, and the norm after a residual sum reads its modulations when the
+    sum is stored: the same tensor there may not be written in place."""
+    q, other = torch.zeros(1, 2, 5, 16), torch.zeros(1, 2, 5, 16)
+    r, y, rms = torch.zeros(2, 3, 16), torch.zeros(2, 3, 16), Norm("rms")
+    one = torch.zeros(1, 16)
+    for call in (lambda: rotate_qk(q, q, out=(q, other)), lambda: rotate_qk(q, q, out=(other, q)),
+                 lambda: gated_residual(r, y, norm=rms, scale=r, out=(r, None)),
+                 lambda: gated_residual(r, y, norm=rms, shift=r, out=(r, None)),
+                 lambda: gated_residual(one, torch.zeros(1, 16), norm=Norm("rms", one), out=(one, None)),
+                 lambda: modulated_norm(one, Norm("rms", one), out=one)):
+        with pytest.raises(ValueError, match="overlap"):
+            call()
+    # where each element is read by the thread that writes it, before it does
+    for call in (lambda: rotate_qk(q, q), lambda: rotate_qk(q, q, out=(other, torch.zeros(1, 2, 5, 16))),
+                 lambda: gated_residual(r, r, r, out=(r, None)), lambda: gated_residual(r, y, y, norm=rms, out=(r, y)),
+                 lambda: gated_residual(r, y, norm=rms, scale=y, shift=y, out=(None, y)),
+                 lambda: modulated_norm(r, rms, scale=r, shift=r, out=r)):
+        with pytest.raises(ValueError, match=CUDA_ONLY):
+            call()

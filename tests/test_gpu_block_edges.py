@@ -205,3 +205,24 @@ def test_text_with_norms_of_its_own(text_first):
         check(joint[:, :, at["video"]], *ref_turn64(qk["video"][i], norms["video"][i], dims, pos, inside, BF))
         y, big = ref_norm64(qk["text"][i].double(), norms["text"][i], (3,))
         check(joint[:, :, at["text"]], y, (27 + 2 * math.sqrt(d)) * U * big)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("s,c", [(3, 64), (2501, 64), (2501, 1352), (2100, 3080), (2050, 4104), (2050, 5120), (2048, 8200),
+                                 (1, 16384), (2048, 16384)])
+def test_one_tensor_in_several_places_written_in_place(dtype, s, c):
+    """The calls that are taken though an input stands in two places and is replaced: the bits of the same calls on copies."""
+    g = _gen(47)
+    norm = row_norm(g, "layer", c, dtype)
+    r0, y0 = rows(g, dtype, 1, s, c), (0.3 * torch.randn(1, s, c, generator=g, device=DEV)).to(dtype)
+
+    def both(call):
+        want = call(r0.clone(), r0.clone(), y0.clone(), y0.clone(), lambda *t: None)
+        r, y = r0.clone(), y0.clone()
+        got = call(r, r, y, y, lambda *t: t)
+        assert all(torch.equal(a, b) for a, b in zip(got, want) if a is not None)
+
+    both(lambda r, r2, y, y2, out: gated_residual(r, r2, r2, norm=norm, out=out(r, None)))
+    both(lambda r, r2, y, y2, out: gated_residual(r, y, y2, norm=norm, scale=y2, shift=y2, out=out(r, y)))
+    both(lambda r, r2, y, y2, out: gated_residual(r, y, norm=norm, scale=y2, shift=y2, out=out(None, y)))
+    both(lambda r, r2, y, y2, out: (modulated_norm(y, norm, scale=y2, shift=y2, out=(out(y) or (None,))[0]),))
