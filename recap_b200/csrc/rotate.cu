@@ -8,8 +8,8 @@
 // with c, s = cos, sin of 2 pi (position[axis p](n) turns_p + phase_p).  The angle is kept in
 // turns as a 64-bit fixed-point fraction: position * turns_p wraps modulo one turn by itself,
 // so the angle of a position of any size is that of turns_p to 2^-32 of a turn, with no table and no
-// reduction of a large float.  (turns_p itself is as good as its maker's: block.py rounds frequencies to 53 bits.)  Values past the turned ones, and tokens outside the grid (text),
-// are only normalised.
+// reduction of a large float.  (turns_p is as good as its maker's: block.py rounds frequencies to 53 bits.)
+// Values past the turned ones, and tokens outside the grid (text), are only normalised.
 //
 // Bound by memory: each row is read once and written once.  A row lies on kLanes lanes (8, 16 or
 // 32 for head dims up to 64, 128 and 256), 16 bytes of bf16 each; those lanes form a group.  A
